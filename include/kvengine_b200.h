@@ -36,7 +36,7 @@ enum {
   KVE_ERR_BOUNDS = -7      /* device side: slot / block / token id out of range */
 };
 
-enum { KVE_F32 = 0, KVE_BF16 = 1 };
+enum { KVE_F32 = 0, KVE_BF16 = 1, KVE_FP8_E4M3 = 2 };  /* FP8_E4M3: caches of the *_fp8 ops only */
 
 /* GEMM epilogues: out[m, :] from acc[m, :] = sum_k x[m,k] * w[n,k].
  *   STORE     out = round(acc)
@@ -356,6 +356,131 @@ int kve_spec_next_draft_plan(const int32_t* start_lens, const int32_t* last_toke
                              const int32_t* tables, int n_seqs, int width, int block_size, int k, int rows,
                              int dump_block, const int32_t* n_accepted, const int32_t* emitted, int32_t* plan_out,
                              int32_t* ids_out, int32_t* verify_ids_out, int* dev_status, cudaStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Speculative decoding with sampling, trees of drafts and an 8-bit cache (no
+ * kvengine counterpart: its drafts are chains, its acceptance greedy
+ * (kvengine/speculative.py:111-216), its pools of the model's dtype
+ * (kvengine/paged.py:59-67)). A step of it: kve_qkv_rope_append_fp8 (or
+ * kve_qkv_rope_append) and kve_paged_tree_attn in every layer,
+ * kve_sample_accept or kve_tree_sample_accept on the logits, and, for a tree,
+ * kve_kv_commit_path. Calls that share a workspace are ordered on one stream
+ * (the graphs that hold them included).
+ * ------------------------------------------------------------------------ */
+
+/* Attention of trees of drafted tokens, of chains and of single tokens over a paged cache.
+ * Sequence b's q_lens[b] new tokens (the nodes of its tree) have their K/V in the
+ * cache behind its history, at positions ctx_lens[b] - q_lens[b] + node. Row `node`
+ * attends all of the history and the nodes t whose bit is set in its mask words:
+ * bit t % 32 of tree_mask[(q_offsets[b] + node) * mask_words + t / 32], t < q_lens[b]
+ * (a node's own bit is not implied; mask_words >= ceil(max_q_len / 32)). tree_mask
+ * NULL: nodes up to itself (a chain). A row that sees no key gets zeros; K and V
+ * of nodes that a row does not see do not reach it, infinities and NaN included.
+ * dtype: of q and out (KVE_BF16 or KVE_F32); kv_dtype: the same, or KVE_FP8_E4M3 for
+ * bf16 queries over a cache written by the *_fp8 ops, with the layer's scale bytes
+ * [num_blocks, block_size, num_kv_heads]. q, out, tables, lengths and offsets as
+ * for kve_paged_verify_attn; head_dim 64 or 128, at most 64 query heads per kv head,
+ * max_q_len <= 1024 (longer prompts: in pieces), ctx_lens[b] <= max_ctx.
+ * Only the rows [q_offsets[b], q_offsets[b] + q_lens[b]) of out are written.
+ * A sequence with inconsistent lengths is skipped, a block id outside the pool reads
+ * as zeros; both record KVE_ERR_BOUNDS. Workspace: zeroed once; as
+ * kve_tree_attn_workspace_bytes says (0: none). */
+size_t kve_tree_attn_workspace_bytes(int batch, int max_q_len, int max_ctx, int num_heads, int num_kv_heads,
+                                     int head_dim);
+int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k, const void* pool_v, int kv_dtype,
+                        const uint8_t* k_scale, const uint8_t* v_scale, const int32_t* block_tables, int table_stride,
+                        const int32_t* ctx_lens, const int32_t* q_lens, const int32_t* q_offsets,
+                        const uint32_t* tree_mask, int mask_words, int batch, int max_q_len, int max_ctx, int num_heads,
+                        int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, float scale, void* out,
+                        void* workspace, size_t workspace_bytes, int* dev_status, cudaStream_t stream);
+
+/* The 8-bit cache. A row (token, kv head, K or V) of head_dim (64 or 128) elements x is
+ * held as e4m3 numbers q = x 2^-e rounded to nearest even, and the byte e + 127,
+ * e being the least integer >= -126 with max|x| <= 448 2^e over the finite elements (0
+ * for a zero row). Infinities and NaN become NaN. pool_k/v: one layer's
+ * [num_slots, num_kv_heads, head_dim] bytes; k/v_scale: [num_slots, num_kv_heads].
+ * Slots of one call are distinct (of two tokens on one slot either, or parts of
+ * both, may be left there); a slot outside [0, num_slots) is skipped (read: zeros) and
+ * reported as KVE_ERR_BOUNDS. All pointers but the scales, slots and positions are
+ * 16-byte aligned.
+ * kve_qkv_rope_append_fp8: kve_qkv_rope_append for such a cache. The rotation is
+ * computed in fp32 and rounded once, to q_out's dtype or to the cache.
+ * kve_kv_append_fp8: kve_kv_append for such a cache (rows already rotated).
+ * kve_kv_read_fp8: rows of given slots as the values they stand for, k_out and v_out
+ * [n_tokens, num_kv_heads, head_dim] in dtype (exact in bf16 and fp32). */
+int kve_qkv_rope_append_fp8(const void* qkv, int dtype, int n_tokens, int num_heads, int num_kv_heads, int head_dim,
+                            const int32_t* positions, const int32_t* slots, const float* rope_cos,
+                            const float* rope_sin, int rope_len, void* q_out, void* pool_k, void* pool_v,
+                            uint8_t* k_scale, uint8_t* v_scale, int64_t num_slots, int* dev_status,
+                            cudaStream_t stream);
+int kve_kv_append_fp8(const void* k_new, const void* v_new, int dtype, const int64_t* slot_ids, int n_tokens,
+                      int num_kv_heads, int head_dim, void* pool_k, void* pool_v, uint8_t* k_scale, uint8_t* v_scale,
+                      int64_t num_slots, int* dev_status, cudaStream_t stream);
+int kve_kv_read_fp8(const void* pool_k, const void* pool_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                    const int64_t* slot_ids, int n_tokens, int num_kv_heads, int head_dim, int64_t num_slots, int dtype,
+                    void* k_out, void* v_out, int* dev_status, cudaStream_t stream);
+
+/* Verification of a chain of k drafts by sampling. With p_j = softmax(logits[b, j] / T),
+ * T = temperature[b], and q_j = softmax(draft_logits[b, j] / T) (draft_logits NULL: a
+ * draft without a distribution, q_j one at draft j): draft j is accepted where
+ * uniforms[b, j] q_j(draft_j) < p_j(draft_j); n is the length of the accepted prefix;
+ * the token behind it is argmax_v(log w_v + gumbel[b, v]), lowest v among equals, with
+ * w = max(p_n - q_n, 0), or p_k where all were accepted, or p_n where no w is positive.
+ * Uniforms in [0, 1) and Gumbel noise -log(-log u) give tokens distributed as sampling
+ * from the target alone. T <= 0 (or NaN): p and q are one-hot at their lowest argmax.
+ * A NaN logit counts as minus infinity; a row without any probability accepts nothing
+ * and gives token 0 with log-probability -inf. A draft outside [0, vocab) is rejected
+ * and recorded as KVE_ERR_BOUNDS.
+ * logits: [batch, k+1, vocab] rows row_stride elements apart (fp32 or bf16); draft_logits
+ * (same dtype): row j of sequence b at b * stride_b + j * stride_j; drafts as for
+ * kve_greedy_accept; uniforms [batch, k] rows uniform_stride_b apart; gumbel
+ * [batch, vocab] fp32 rows gumbel_stride apart; temperature [batch] fp32. 1 <= k <= 31.
+ * Outputs: n_accepted [batch], emitted [batch, k+1] (drafts[:n], the token drawn, -1), and
+ * logprobs [batch, k+1]: log p of each emitted token (0 for T <= 0 and past the end). */
+size_t kve_sample_accept_workspace_bytes(int batch, int k, int vocab, int with_draft_logits);
+int kve_sample_accept(const void* logits, int dtype, int64_t row_stride, const void* draft_logits,
+                      int64_t draft_logits_stride_b, int64_t draft_logits_stride_j, const int32_t* drafts,
+                      int64_t draft_stride_b, int64_t draft_stride_j, const float* uniforms, int64_t uniform_stride_b,
+                      const float* gumbel, int64_t gumbel_stride, const float* temperature, int batch, int k, int vocab,
+                      int32_t* out_n_accepted, int32_t* out_emitted, float* out_logprobs, void* workspace,
+                      size_t workspace_bytes, int* dev_status, cudaStream_t stream);
+
+/* Verification of trees of candidate tokens by sampling. Sequence b's tree has q_lens[b]
+ * nodes, rows q_offsets[b] .. of logits [n_rows, vocab], tokens, parents and uniforms
+ * [n_rows]; q_offsets [batch] ascends. Node 0 is the token before the tree (its
+ * logits predict its children; its token, parent and uniform are not read); the
+ * others have 0 <= parent < their own index. From node 0: the children of the
+ * current node in index order, child c with token d accepted (and then current)
+ * where uniforms[c] R < p(d), R = 1 - sum of p over the siblings rejected before it, p
+ * being 0 for a token rejected before at this node. Where no child is left, the last
+ * token is argmax_v(log p_v + gumbel[b, v]) over the tokens not rejected there (over all,
+ * where those have no probability). p, T, NaN and the noise as for kve_sample_accept.
+ * A node with a token or parent out of range is nobody's child and recorded as
+ * KVE_ERR_BOUNDS. max_q_len <= 1024.
+ * Outputs: n_accepted [batch] (-1 for a sequence without nodes, whose other outputs
+ * are not written), and, [batch, max_q_len]: path (the accepted nodes, node 0 first, then
+ * -1), emitted (their tokens without node 0's, the token drawn, then -1), logprobs. */
+size_t kve_tree_sample_accept_workspace_bytes(int n_rows, int vocab);
+int kve_tree_sample_accept(const void* logits, int dtype, int64_t row_stride, const int32_t* tokens,
+                           const int32_t* parents, const int32_t* q_lens, const int32_t* q_offsets,
+                           const float* uniforms, const float* gumbel, int64_t gumbel_stride, const float* temperature,
+                           int batch, int n_rows, int max_q_len, int vocab, int32_t* out_n_accepted, int32_t* out_path,
+                           int32_t* out_emitted, float* out_logprobs, void* workspace, size_t workspace_bytes,
+                           int* dev_status, cudaStream_t stream);
+
+/* The accepted path's K/V moved together in every layer: for j = 1 .. n_accepted[b], the
+ * row of position start_lens[b] + path[b, j] goes to position start_lens[b] + j, in order.
+ * path: [batch, path_stride] (<= 1024), path[b, 0] is node 0 and the others ascend, as
+ * kve_tree_sample_accept writes them; start_lens[b]: the position of node 0. The caller
+ * then keeps start + n_accepted + 1 positions. pools: [num_layers, num_blocks,
+ * block_size, num_kv_heads, head_dim] of kv_dtype (rows of a multiple of 16 bytes), with
+ * their scales [num_layers, num_blocks, block_size, num_kv_heads] for KVE_FP8_E4M3 (else
+ * NULL). n_accepted 0 or -1: nothing moves. A sequence whose path does not ascend or
+ * leaves its table is skipped and recorded as KVE_ERR_BOUNDS. */
+int kve_kv_commit_path(void* pool_k, void* pool_v, int kv_dtype, uint8_t* k_scale, uint8_t* v_scale, int num_layers,
+                       int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, const int32_t* block_tables,
+                       int table_stride, const int32_t* start_lens, const int32_t* path, int path_stride,
+                       const int32_t* n_accepted, int batch, int* dev_status, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

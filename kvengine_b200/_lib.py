@@ -19,7 +19,7 @@ KVE_ERR = {
     -1: "KVE_ERR_ARG", -2: "KVE_ERR_SHAPE", -3: "KVE_ERR_DTYPE", -4: "KVE_ERR_CUDA",
     -5: "KVE_ERR_TIMEOUT", -6: "KVE_ERR_WORKSPACE", -7: "KVE_ERR_BOUNDS",
 }
-KVE_F32, KVE_BF16 = 0, 1
+KVE_F32, KVE_BF16, KVE_FP8_E4M3 = 0, 1, 2
 EPI_STORE, EPI_BIAS, EPI_RESIDUAL, EPI_SILU_MUL = 0, 1, 2, 3
 GEMM_AUTO, GEMM_SIMT, GEMM_TCGEN05 = 0, 1, 2
 
@@ -95,6 +95,20 @@ _SIGNATURES = {
     "kve_forward_layers": (i32, [C.POINTER(ModelT), C.POINTER(BatchT), C.POINTER(ScratchT), i32, i32, vp]),
     "kve_forward_layers_graphed": (i32, [C.POINTER(ModelT), C.POINTER(BatchT), C.POINTER(ScratchT), i32, i32,
                                          C.POINTER(C.c_void_p), vp]),
+    "kve_tree_attn_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+    "kve_paged_tree_attn": (i32, [vp, i32, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32,
+                                  i32, i32, i64, f32, vp, vp, sz, vp, vp]),
+    "kve_qkv_rope_append_fp8": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, i64, vp,
+                                      vp]),
+    "kve_kv_append_fp8": (i32, [vp, vp, i32, vp, i32, i32, i32, vp, vp, vp, vp, i64, vp, vp]),
+    "kve_kv_read_fp8": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i64, i32, vp, vp, vp, vp]),
+    "kve_sample_accept_workspace_bytes": (sz, [i32, i32, i32, i32]),
+    "kve_sample_accept": (i32, [vp, i32, i64, vp, i64, i64, vp, i64, i64, vp, i64, vp, i64, vp, i32, i32, i32, vp, vp,
+                                vp, vp, sz, vp, vp]),
+    "kve_tree_sample_accept_workspace_bytes": (sz, [i32, i32]),
+    "kve_tree_sample_accept": (i32, [vp, i32, i64, vp, vp, vp, vp, vp, vp, i64, vp, i32, i32, i32, i32, vp, vp, vp, vp,
+                                     vp, sz, vp, vp]),
+    "kve_kv_commit_path": (i32, [vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp, i32, vp, vp, i32, vp, i32, vp, vp]),
     "kve_spec_next_draft_plan": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]),
 }
 

@@ -12,6 +12,13 @@ attention reads blocks in place (`kve_paged_verify_attn`). `write` still
 returns the gathered history for callers of the KVCacheLike protocol.
 `truncate` is pure block-table bookkeeping, exactly like the reference: no
 data moves, whole trailing blocks go back to the allocator.
+
+A pool of dtype torch.float8_e4m3fn is the 8-bit cache: k and v hold e4m3
+numbers and k_scale, v_scale [num_layers, num_blocks, block_size, num_kv_heads]
+uint8 a power of two per row (exponent + 127). `write` quantises
+(`kve_kv_append_fp8`) and returns the history as it is read back, in the given
+rows' dtype; `ops.tree_attention` reads such a pool in place. The fused model
+pass (`Runner`) takes pools of the model's dtype only.
 """
 
 from __future__ import annotations
@@ -39,6 +46,10 @@ class PagedKVCache:
         self.k = torch.zeros(shape, dtype=dtype, device=self.device)
         self.v = torch.zeros(shape, dtype=dtype, device=self.device)
         flat = (num_layers, num_blocks * block_size, num_kv_heads, head_dim)
+        self.k_scale = self.v_scale = None
+        if dtype == torch.float8_e4m3fn:  # the 8-bit cache: a zero row has exponent 0
+            self.k_scale = torch.full(shape[:-1], 127, dtype=torch.uint8, device=self.device)
+            self.v_scale = torch.full(shape[:-1], 127, dtype=torch.uint8, device=self.device)
         self.k_flat = self.k.view(flat)
         self.v_flat = self.v.view(flat)
         self.manager = BlockManager(num_blocks, block_size)
@@ -53,7 +64,8 @@ class PagedKVCache:
         return cls(c.num_layers, c.num_kv_heads, c.head_dim, num_blocks, block_size, m.dtype, m.device)
 
     def nbytes(self) -> int:
-        return self.k.numel() * self.k.element_size() * 2
+        scales = 0 if self.k_scale is None else self.k_scale.numel() * 2
+        return self.k.numel() * self.k.element_size() * 2 + scales
 
     def bytes_per_block(self) -> int:
         return self.nbytes() // self.num_blocks
@@ -155,6 +167,12 @@ class PagedSequenceCache:
         slots = torch.tensor(self.slot_list(start, n), dtype=torch.long, device=self.pool.device)
         k_src = k[0].transpose(0, 1).contiguous()
         v_src = v[0].transpose(0, 1).contiguous()
+        if self.pool.k_scale is not None:
+            cache = (self.pool.k[layer_idx], self.pool.v[layer_idx], self.pool.k_scale[layer_idx],
+                     self.pool.v_scale[layer_idx])
+            ops.kv_append_fp8(k_src, v_src, slots, *cache)
+            k_all, v_all = ops.kv_read_fp8(*cache, self.slot_indices(0, start + n), dtype=k.dtype)
+            return k_all.transpose(0, 1)[None], v_all.transpose(0, 1)[None]
         ops.kv_append(k_src, v_src, slots, self.pool.k[layer_idx], self.pool.v[layer_idx])
         return self._gather(layer_idx, start + n)
 
