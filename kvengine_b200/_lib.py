@@ -162,6 +162,10 @@ def stream_handle(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The current stream of a device by its index, without building a Stream object (2 us a call).
+raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:

@@ -7,6 +7,8 @@ caller keeps (the kernels leave them zeroed).
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib as L
@@ -236,28 +238,62 @@ def spec_next_draft_plan(start_lens: torch.Tensor, last_tokens: torch.Tensor, n_
 
 
 # ------------------------------------------------ sampling, draft trees and the 8-bit cache
-def _like(name: str, dev: torch.device, **tensors) -> None:
-    """Every given (tensor, dtype, shape) is a contiguous tensor of that dtype and shape on `dev`
-    (a shape of None: any)."""
-    for what, (t, dtype, shape) in tensors.items():
-        if t.dtype != dtype or t.device != dev or not t.is_contiguous() or (shape is not None and t.shape != shape):
-            raise ValueError(f"{name}: {what} must be a contiguous {dtype} tensor"
-                             f"{'' if shape is None else ' ' + str(list(shape))} on {dev}, got {t.dtype} {list(t.shape)} "
-                             f"with strides {t.stride()} on {t.device}")
+# These calls are a few microseconds of GPU work in a decode step, so their checks are
+# kept to a few attribute reads per tensor and the message is made only for a failure.
+_I32, _F32, _U8, _E4M3 = torch.int32, torch.float32, torch.uint8, torch.float8_e4m3fn
 
 
-def _call(fn, dev: torch.device, *args) -> None:
-    """fn(*args, stream) on the current stream of `dev`, which is made current if it is not."""
-    if dev.index == torch.cuda.current_device():
-        L.check(fn(*args, L.stream_handle(dev)))
+def _refuse(name: str, rule: str) -> None:
+    raise ValueError(f"{name}: {rule}")
+
+
+def _dense(name: str, index: int, *tensors) -> None:
+    """Every (tensor, dtype) is a contiguous tensor of that dtype on CUDA device `index`."""
+    for at, (t, dtype) in enumerate(tensors):
+        if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+            _refuse(name, f"tensor {at + 1} of {len(tensors)} checked together must be contiguous {dtype} on cuda:{index}, "
+                          f"got {t.dtype} {list(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _device(t: torch.Tensor) -> int:
+    index = t.get_device()
+    if index < 0:
+        L.require_cuda(t)
+    return index
+
+
+def _call(fn, index: int, *args) -> None:
+    """fn(*args, stream) on the current stream of device `index`, which is made current if it is not."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, L.raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            L.check(fn(*args, L.stream_handle(dev)))
+        with torch.cuda.device(index):
+            rc = fn(*args, L.raw_stream(index))
+    if rc:
+        L.check(rc)
 
 
-def _fp8_cache(name: str, dev, k, v, k_scale, v_scale) -> None:
-    _like(name, dev, pool_k=(k, torch.float8_e4m3fn, None), pool_v=(v, torch.float8_e4m3fn, k.shape),
-          k_scale=(k_scale, torch.uint8, k.shape[:-1]), v_scale=(v_scale, torch.uint8, k.shape[:-1]))
+def _fp8_cache(name: str, index: int, k, v, k_scale, v_scale) -> None:
+    _dense(name, index, (k, _E4M3), (v, _E4M3), (k_scale, _U8), (v_scale, _U8))
+    shape = k.shape
+    if v.shape != shape or k_scale.shape != shape[:-1] or v_scale.shape != shape[:-1]:
+        _refuse(name, f"caches and scales of different shapes: {list(shape)}, {list(v.shape)}, {list(k_scale.shape)}, "
+                      f"{list(v_scale.shape)}")
+
+
+@lru_cache(maxsize=4096)
+def _tree_attn_ws(*sizes: int) -> int:
+    return L.load().kve_tree_attn_workspace_bytes(*sizes)
+
+
+@lru_cache(maxsize=4096)
+def _sample_ws(*sizes: int) -> int:
+    return L.load().kve_sample_accept_workspace_bytes(*sizes)
+
+
+@lru_cache(maxsize=4096)
+def _tree_sample_ws(*sizes: int) -> int:
+    return L.load().kve_tree_sample_accept_workspace_bytes(*sizes)
 
 
 def tree_attention(q, pool_k_layer, pool_v_layer, block_tables, ctx_lens, q_lens, q_offsets, max_q_len: int, max_ctx: int,
@@ -269,47 +305,48 @@ def tree_attention(q, pool_k_layer, pool_v_layer, block_tables, ctx_lens, q_lens
     chain); a row that sees nothing gets zeros. bf16 queries also read an e4m3 cache, given
     its layer's k_scale and v_scale [num_blocks, bs, nkv] uint8."""
     lib = L.load()
-    L.require_cuda(q)
-    dev = q.device
+    dev = _device(q)
     n, nq, hd = q.shape
     num_blocks, bs, nkv, pool_hd = pool_k_layer.shape
-    B = ctx_lens.shape[0]
-    if pool_hd != hd:
-        raise ValueError(f"tree_attention: head_dim {hd} of q, {pool_hd} of the cache")
+    B, width = block_tables.shape
+    dtype = q.dtype
+    code = L.dtype_code(dtype)
     if k_scale is None and v_scale is None:
-        kv_code = L.dtype_code(q.dtype)
-        _like("tree_attention", dev, q=(q, q.dtype, None), pool_k=(pool_k_layer, q.dtype, None),
-              pool_v=(pool_v_layer, q.dtype, pool_k_layer.shape))
+        kv_code, ks, vs = code, None, None
+        _dense("tree_attention", dev, (q, dtype), (pool_k_layer, dtype), (pool_v_layer, dtype), (block_tables, _I32),
+               (ctx_lens, _I32), (q_lens, _I32), (q_offsets, _I32))
     else:
-        kv_code = L.KVE_FP8_E4M3
         if k_scale is None or v_scale is None:
-            raise ValueError("tree_attention: k_scale and v_scale go together")
-        _like("tree_attention", dev, q=(q, torch.bfloat16, None))
+            _refuse("tree_attention", "k_scale and v_scale go together")
+        kv_code, ks, vs = L.KVE_FP8_E4M3, k_scale.data_ptr(), v_scale.data_ptr()
+        _dense("tree_attention", dev, (q, torch.bfloat16), (block_tables, _I32), (ctx_lens, _I32), (q_lens, _I32),
+               (q_offsets, _I32))
         _fp8_cache("tree_attention", dev, pool_k_layer, pool_v_layer, k_scale, v_scale)
-    i32 = torch.int32
-    _like("tree_attention", dev, block_tables=(block_tables, i32, None), ctx_lens=(ctx_lens, i32, None),
-          q_lens=(q_lens, i32, ctx_lens.shape), q_offsets=(q_offsets, i32, None))
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or q_offsets.shape[0] < B:
-        raise ValueError("tree_attention: one block table row, length and offset per sequence")
-    words = 0
+    if pool_hd != hd or pool_v_layer.shape != pool_k_layer.shape:
+        _refuse("tree_attention", f"head_dim {hd} of q, caches {list(pool_k_layer.shape)} and {list(pool_v_layer.shape)}")
+    if ctx_lens.numel() != B or q_lens.numel() != B or q_offsets.numel() < B:
+        _refuse("tree_attention", "one block table row, length and offset per sequence")
+    mask, words = None, 0
     if tree_mask is not None:
-        _like("tree_attention", dev, tree_mask=(tree_mask, i32, None))
-        if tree_mask.dim() != 2 or tree_mask.shape[0] != n:
-            raise ValueError("tree_attention: one tree_mask row per row of q")
-        words = tree_mask.shape[1]
+        _dense("tree_attention", dev, (tree_mask, _I32))
+        rows, words = tree_mask.shape
+        if rows != n:
+            _refuse("tree_attention", "one tree_mask row per row of q")
+        mask = tree_mask.data_ptr()
     if out is None:
         out = torch.empty_like(q)
     else:
-        _like("tree_attention", dev, out=(out, q.dtype, q.shape))
-    need = lib.kve_tree_attn_workspace_bytes(B, max_q_len, max_ctx, nq, nkv, hd)
+        _dense("tree_attention", dev, (out, dtype))
+        if out.shape != q.shape:
+            _refuse("tree_attention", "out has the shape of q")
+    need = _tree_attn_ws(B, max_q_len, max_ctx, nq, nkv, hd)
     ws, ws_bytes = None, 0
     if need:
-        buf = (workspace or Workspace(dev)).get(need)
+        buf = (workspace or Workspace(q.device)).get(need)
         ws, ws_bytes = buf.data_ptr(), buf.numel()
-    _call(lib.kve_paged_tree_attn, dev, q.data_ptr(), L.dtype_code(q.dtype), pool_k_layer.data_ptr(), pool_v_layer.data_ptr(),
-          kv_code, L.ptr(k_scale), L.ptr(v_scale), block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(),
-          q_lens.data_ptr(), q_offsets.data_ptr(), L.ptr(tree_mask), words, B, max_q_len, max_ctx, nq, nkv, hd, bs,
-          num_blocks, scale, out.data_ptr(), ws, ws_bytes, L.ptr(status))
+    _call(lib.kve_paged_tree_attn, dev, q.data_ptr(), code, pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), kv_code, ks, vs,
+          block_tables.data_ptr(), width, ctx_lens.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(), mask, words, B,
+          max_q_len, max_ctx, nq, nkv, hd, bs, num_blocks, scale, out.data_ptr(), ws, ws_bytes, L.ptr(status))
     return out
 
 
@@ -337,39 +374,39 @@ def qkv_rope_append_fp8(qkv, positions, slots, rope_cos, rope_sin, q_out, pool_k
     """`qkv_rope_append` into an e4m3 cache (pools [num_blocks, bs, nkv, hd] float8_e4m3fn, scales
     [num_blocks, bs, nkv] uint8): q rotated into q_out, K rotated and quantised, V quantised."""
     lib = L.load()
-    L.require_cuda(qkv)
-    dev, n = qkv.device, qkv.shape[0]
     name = "qkv_rope_append_fp8"
-    _like(name, dev, qkv=(qkv, qkv.dtype, (n, (num_heads + 2 * num_kv_heads) * head_dim)),
-          positions=(positions, torch.int32, (n,)), slots=(slots, torch.int32, (n,)),
-          rope_cos=(rope_cos, torch.float32, (rope_cos.shape[0], head_dim // 2)),
-          rope_sin=(rope_sin, torch.float32, rope_cos.shape))
-    if q_out.numel() != n * num_heads * head_dim:
-        raise ValueError(f"{name}: q_out must have n_tokens x num_heads x head_dim elements")
-    _like(name, dev, q_out=(q_out, qkv.dtype, None))
+    dev, dtype = _device(qkv), qkv.dtype
+    n, width = qkv.shape
+    _dense(name, dev, (qkv, dtype), (positions, _I32), (slots, _I32), (rope_cos, _F32), (rope_sin, _F32), (q_out, dtype))
     _fp8_cache(name, dev, pool_k_layer, pool_v_layer, k_scale, v_scale)
-    if pool_k_layer.shape[2:] != (num_kv_heads, head_dim):
-        raise ValueError(f"{name}: the cache has heads {list(pool_k_layer.shape[2:])}")
-    _call(lib.kve_qkv_rope_append_fp8, dev, qkv.data_ptr(), L.dtype_code(qkv.dtype), n, num_heads, num_kv_heads, head_dim,
-          positions.data_ptr(), slots.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0],
-          q_out.data_ptr(), pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-          pool_k_layer.shape[0] * pool_k_layer.shape[1], L.ptr(status))
+    num_blocks, bs, nkv, hd = pool_k_layer.shape
+    rope_len, half = rope_cos.shape
+    if width != (num_heads + 2 * num_kv_heads) * head_dim or nkv != num_kv_heads or hd != head_dim or \
+            positions.numel() != n or slots.numel() != n or half * 2 != hd or rope_sin.shape != rope_cos.shape or \
+            q_out.numel() != n * num_heads * head_dim:
+        _refuse(name, f"shapes do not fit {num_heads}/{num_kv_heads} heads of {head_dim}: qkv {list(qkv.shape)}, positions "
+                      f"{list(positions.shape)}, slots {list(slots.shape)}, tables {list(rope_cos.shape)} "
+                      f"{list(rope_sin.shape)}, q_out {list(q_out.shape)}, cache {list(pool_k_layer.shape)}")
+    _call(lib.kve_qkv_rope_append_fp8, dev, qkv.data_ptr(), L.dtype_code(dtype), n, num_heads, num_kv_heads, head_dim,
+          positions.data_ptr(), slots.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), rope_len, q_out.data_ptr(),
+          pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks * bs,
+          L.ptr(status))
 
 
 def kv_append_fp8(k_new, v_new, slot_ids, pool_k_layer, pool_v_layer, k_scale, v_scale, status=None) -> None:
     """`kv_append` into an e4m3 cache: rows [n, nkv, hd] quantised, each with its own power of two."""
     lib = L.load()
-    L.require_cuda(k_new)
-    dev = k_new.device
+    dev, dtype = _device(k_new), k_new.dtype
     n, nkv, hd = k_new.shape
-    _like("kv_append_fp8", dev, k_new=(k_new, k_new.dtype, None), v_new=(v_new, k_new.dtype, k_new.shape),
-          slot_ids=(slot_ids, torch.int64, (n,)))
+    _dense("kv_append_fp8", dev, (k_new, dtype), (v_new, dtype), (slot_ids, torch.int64))
     _fp8_cache("kv_append_fp8", dev, pool_k_layer, pool_v_layer, k_scale, v_scale)
-    if pool_k_layer.shape[2:] != (nkv, hd):
-        raise ValueError(f"kv_append_fp8: the cache has heads {list(pool_k_layer.shape[2:])}")
-    _call(lib.kve_kv_append_fp8, dev, k_new.data_ptr(), v_new.data_ptr(), L.dtype_code(k_new.dtype), slot_ids.data_ptr(), n,
-          nkv, hd, pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-          pool_k_layer.shape[0] * pool_k_layer.shape[1], L.ptr(status))
+    num_blocks, bs, *heads = pool_k_layer.shape
+    if heads != [nkv, hd] or v_new.shape != k_new.shape or slot_ids.numel() != n:
+        _refuse("kv_append_fp8", f"rows {list(k_new.shape)} and {list(v_new.shape)}, {slot_ids.numel()} slots, cache "
+                                 f"{list(pool_k_layer.shape)}")
+    _call(lib.kve_kv_append_fp8, dev, k_new.data_ptr(), v_new.data_ptr(), L.dtype_code(dtype), slot_ids.data_ptr(), n, nkv,
+          hd, pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks * bs,
+          L.ptr(status))
 
 
 def kv_read_fp8(pool_k_layer, pool_v_layer, k_scale, v_scale, slot_ids, dtype: torch.dtype = torch.bfloat16, out=None,
@@ -377,28 +414,34 @@ def kv_read_fp8(pool_k_layer, pool_v_layer, k_scale, v_scale, slot_ids, dtype: t
     """Rows of an e4m3 cache as the values they stand for: (k, v), each [n, nkv, hd] in `dtype`, of
     the flat slots slot_ids [n] int64. `out` may give the two."""
     lib = L.load()
-    L.require_cuda(pool_k_layer)
-    dev = pool_k_layer.device
+    dev = _device(pool_k_layer)
     num_blocks, bs, nkv, hd = pool_k_layer.shape
-    n = slot_ids.shape[0]
     _fp8_cache("kv_read_fp8", dev, pool_k_layer, pool_v_layer, k_scale, v_scale)
-    _like("kv_read_fp8", dev, slot_ids=(slot_ids, torch.int64, (n,)))
+    _dense("kv_read_fp8", dev, (slot_ids, torch.int64))
+    (n,) = slot_ids.shape
     if out is None:
-        k = torch.empty(n, nkv, hd, dtype=dtype, device=dev)
+        k = torch.empty(n, nkv, hd, dtype=dtype, device=pool_k_layer.device)
         v = torch.empty_like(k)
     else:
         k, v = out
-        _like("kv_read_fp8", dev, k_out=(k, dtype, (n, nkv, hd)), v_out=(v, dtype, (n, nkv, hd)))
+        _dense("kv_read_fp8", dev, (k, dtype), (v, dtype))
+        if k.shape != (n, nkv, hd) or v.shape != (n, nkv, hd):
+            _refuse("kv_read_fp8", f"out must be two tensors [{n}, {nkv}, {hd}]")
     _call(lib.kve_kv_read_fp8, dev, pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
           slot_ids.data_ptr(), n, nkv, hd, num_blocks * bs, L.dtype_code(dtype), k.data_ptr(), v.data_ptr(), L.ptr(status))
     return k, v
 
 
-def _noise(name: str, dev, gumbel, temperature, B: int, V: int) -> None:
-    _like(name, dev, temperature=(temperature, torch.float32, (B,)))
-    if gumbel.dtype != torch.float32 or gumbel.shape != (B, V) or gumbel.device != dev or \
-            (V > 1 and gumbel.stride(1) != 1) or (B > 1 and gumbel.stride(0) < V):
-        raise ValueError(f"{name}: gumbel must be float32 [{B}, {V}] on {dev} with unit column stride")
+def _rows(name: str, what: str, index: int, t: torch.Tensor, dtype, rows: int, cols: int) -> int:
+    """The row stride of a [rows, cols] matrix with unit column stride on device `index`."""
+    if t.dtype is not dtype or t.get_device() != index or t.shape != (rows, cols):
+        _refuse(name, f"{what} must be {dtype} [{rows}, {cols}] on cuda:{index}, got {t.dtype} {list(t.shape)} on {t.device}")
+    if t.is_contiguous():
+        return cols
+    stride, unit = t.stride()
+    if (cols > 1 and unit != 1) or (rows > 1 and stride < cols):
+        _refuse(name, f"{what} needs unit column stride and rows apart, got strides {t.stride()}")
+    return max(stride, cols)
 
 
 def sample_accept(logits: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Tensor, gumbel: torch.Tensor,
@@ -409,38 +452,44 @@ def sample_accept(logits: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Te
     (0: greedy), draft_logits [B, k, V] (None: drafts without a distribution) ->
     (n_accepted [B], emitted [B, k+1], logprobs [B, k+1]). `out` may give the three."""
     lib = L.load()
-    L.require_cuda(logits)
-    dev = logits.device
+    name = "sample_accept"
+    dev, dtype = _device(logits), logits.dtype
     B, kp1, V = logits.shape
     k = kp1 - 1
-    if drafts.dtype != torch.int32 or drafts.shape != (B, k) or drafts.device != dev:
-        raise ValueError(f"sample_accept: drafts must be int32 [{B}, {k}] on {dev}")
-    if logits.stride(2) != 1 or (B > 1 and logits.stride(0) != kp1 * logits.stride(1)):
-        raise ValueError("sample_accept: logits rows must be evenly strided with unit column stride")
-    if uniforms.dtype != torch.float32 or uniforms.shape != (B, k) or uniforms.device != dev or \
-            (k > 1 and uniforms.stride(1) != 1) or (B > 1 and uniforms.stride(0) < k):
-        raise ValueError(f"sample_accept: uniforms must be float32 [{B}, {k}] on {dev} with unit column stride")
-    _noise("sample_accept", dev, gumbel, temperature, B, V)
-    dsb = dsj = 0
+    if drafts.dtype is not _I32 or drafts.shape != (B, k) or drafts.get_device() != dev:
+        _refuse(name, f"drafts must be int32 [{B}, {k}] on cuda:{dev}")
+    stride = V
+    if not logits.is_contiguous():
+        sb, stride, unit = logits.stride()
+        if (V > 1 and unit != 1) or (B > 1 and sb != kp1 * stride) or stride < V:
+            _refuse(name, "logits rows must be evenly strided with unit column stride")
+    usb = _rows(name, "uniforms", dev, uniforms, _F32, B, k)
+    gs = _rows(name, "gumbel", dev, gumbel, _F32, B, V)
+    _dense(name, dev, (temperature, _F32))
+    if temperature.numel() != B:
+        _refuse(name, f"temperature must have {B} elements")
+    dl, dlb, dlj = None, 0, 0
     if draft_logits is not None:
-        if draft_logits.dtype != logits.dtype or draft_logits.shape != (B, k, V) or draft_logits.device != dev or \
-                (V > 1 and draft_logits.stride(2) != 1):
-            raise ValueError(f"sample_accept: draft_logits must be {logits.dtype} [{B}, {k}, {V}] on {dev} with unit column "
-                             "stride")
-        dsb, dsj = draft_logits.stride(0), draft_logits.stride(1)
+        dlb, dlj, unit = draft_logits.stride()
+        if draft_logits.dtype is not dtype or draft_logits.shape != (B, k, V) or draft_logits.get_device() != dev or \
+                (V > 1 and unit != 1):
+            _refuse(name, f"draft_logits must be {dtype} [{B}, {k}, {V}] on cuda:{dev} with unit column stride")
+        dl = draft_logits.data_ptr()
     if out is None:
-        n_acc = torch.empty(B, dtype=torch.int32, device=dev)
-        emitted = torch.empty(B, kp1, dtype=torch.int32, device=dev)
-        logprobs = torch.empty(B, kp1, dtype=torch.float32, device=dev)
+        device = logits.device
+        n_acc = torch.empty(B, dtype=_I32, device=device)
+        emitted = torch.empty(B, kp1, dtype=_I32, device=device)
+        logprobs = torch.empty(B, kp1, dtype=_F32, device=device)
     else:
         n_acc, emitted, logprobs = out
-        _like("sample_accept", dev, n_accepted=(n_acc, torch.int32, (B,)), emitted=(emitted, torch.int32, (B, kp1)),
-              logprobs=(logprobs, torch.float32, (B, kp1)))
-    ws = (workspace or Workspace(dev)).get(lib.kve_sample_accept_workspace_bytes(B, k, V, draft_logits is not None))
-    _call(lib.kve_sample_accept, dev, logits.data_ptr(), L.dtype_code(logits.dtype), max(logits.stride(1), V),
-          L.ptr(draft_logits), dsb, dsj, drafts.data_ptr(), drafts.stride(0), drafts.stride(1), uniforms.data_ptr(),
-          max(uniforms.stride(0), k), gumbel.data_ptr(), max(gumbel.stride(0), V), temperature.data_ptr(), B, k, V,
-          n_acc.data_ptr(), emitted.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), ws.numel(), L.ptr(status))
+        _dense(name, dev, (n_acc, _I32), (emitted, _I32), (logprobs, _F32))
+        if n_acc.numel() != B or emitted.shape != (B, kp1) or logprobs.shape != (B, kp1):
+            _refuse(name, f"out must be [{B}], [{B}, {kp1}] and [{B}, {kp1}]")
+    ws = (workspace or Workspace(logits.device)).get(_sample_ws(B, k, V, int(dl is not None)))
+    dsb, dsj = drafts.stride()
+    _call(lib.kve_sample_accept, dev, logits.data_ptr(), L.dtype_code(dtype), stride, dl, dlb, dlj, drafts.data_ptr(), dsb,
+          dsj, uniforms.data_ptr(), usb, gumbel.data_ptr(), gs, temperature.data_ptr(), B, k, V, n_acc.data_ptr(),
+          emitted.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), ws.numel(), L.ptr(status))
     return n_acc, emitted, logprobs
 
 
@@ -453,34 +502,34 @@ def tree_sample_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torc
     q_lens[b] (parents within the tree, node 0 its root); gumbel [B, V], temperature [B] ->
     (n_accepted [B], path, emitted, logprobs [B, max_q_len]). `out` may give the four."""
     lib = L.load()
-    L.require_cuda(logits)
-    dev = logits.device
-    N, V = logits.shape
-    B = q_lens.shape[0]
     name = "tree_sample_accept"
-    if (V > 1 and logits.stride(1) != 1) or (N > 1 and logits.stride(0) < V):
-        raise ValueError(f"{name}: logits needs unit column stride")
-    i32, f32 = torch.int32, torch.float32
-    _like(name, dev, tokens=(tokens, i32, (N,)), parents=(parents, i32, (N,)), uniforms=(uniforms, f32, (N,)),
-          q_lens=(q_lens, i32, (B,)), q_offsets=(q_offsets, i32, None))
-    if q_offsets.shape[0] < B:
-        raise ValueError(f"{name}: one offset per sequence")
-    _noise(name, dev, gumbel, temperature, B, V)
+    dev, dtype = _device(logits), logits.dtype
+    N, V = logits.shape
+    B = q_lens.numel()
+    stride = _rows(name, "logits", dev, logits, dtype, N, V)
+    gs = _rows(name, "gumbel", dev, gumbel, _F32, B, V)
+    _dense(name, dev, (tokens, _I32), (parents, _I32), (uniforms, _F32), (q_lens, _I32), (q_offsets, _I32),
+           (temperature, _F32))
+    if tokens.numel() != N or parents.numel() != N or uniforms.numel() != N or q_offsets.numel() < B or \
+            temperature.numel() != B:
+        _refuse(name, f"{N} rows need as many tokens, parents and uniforms, {B} sequences as many offsets and temperatures")
     if out is None:
-        n_acc = torch.empty(B, dtype=i32, device=dev)
-        path = torch.empty(B, max_q_len, dtype=i32, device=dev)
+        device = logits.device
+        n_acc = torch.empty(B, dtype=_I32, device=device)
+        path = torch.empty(B, max_q_len, dtype=_I32, device=device)
         emitted = torch.empty_like(path)
-        logprobs = torch.empty(B, max_q_len, dtype=f32, device=dev)
+        logprobs = torch.empty(B, max_q_len, dtype=_F32, device=device)
     else:
         n_acc, path, emitted, logprobs = out
+        _dense(name, dev, (n_acc, _I32), (path, _I32), (emitted, _I32), (logprobs, _F32))
         shape = (B, max_q_len)
-        _like(name, dev, n_accepted=(n_acc, i32, (B,)), path=(path, i32, shape), emitted=(emitted, i32, shape),
-              logprobs=(logprobs, f32, shape))
-    ws = (workspace or Workspace(dev)).get(lib.kve_tree_sample_accept_workspace_bytes(N, V))
-    _call(lib.kve_tree_sample_accept, dev, logits.data_ptr(), L.dtype_code(logits.dtype), max(logits.stride(0), V),
-          tokens.data_ptr(), parents.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(), uniforms.data_ptr(),
-          gumbel.data_ptr(), max(gumbel.stride(0), V), temperature.data_ptr(), B, N, max_q_len, V, n_acc.data_ptr(),
-          path.data_ptr(), emitted.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), ws.numel(), L.ptr(status))
+        if n_acc.numel() != B or path.shape != shape or emitted.shape != shape or logprobs.shape != shape:
+            _refuse(name, f"out must be [{B}] and three times [{B}, {max_q_len}]")
+    ws = (workspace or Workspace(logits.device)).get(_tree_sample_ws(N, V))
+    _call(lib.kve_tree_sample_accept, dev, logits.data_ptr(), L.dtype_code(dtype), stride, tokens.data_ptr(),
+          parents.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(), uniforms.data_ptr(), gumbel.data_ptr(), gs,
+          temperature.data_ptr(), B, N, max_q_len, V, n_acc.data_ptr(), path.data_ptr(), emitted.data_ptr(),
+          logprobs.data_ptr(), ws.data_ptr(), ws.numel(), L.ptr(status))
     return n_acc, path, emitted, logprobs
 
 
@@ -491,22 +540,24 @@ def kv_commit_path(pool_k, pool_v, block_tables, start_lens, path, n_accepted, k
     nkv, hd] (an e4m3 cache with its scales [L, num_blocks, bs, nkv]); path [B, P] and n_accepted
     [B] int32 as `tree_sample_accept` gives them; start_lens [B] the positions of the trees' node 0."""
     lib = L.load()
-    L.require_cuda(pool_k)
-    dev = pool_k.device
+    dev = _device(pool_k)
     layers, num_blocks, bs, nkv, hd = pool_k.shape
-    B, i32 = start_lens.shape[0], torch.int32
+    B, width = block_tables.shape
+    path_rows, path_width = path.shape
     if k_scale is None and v_scale is None:
-        code = L.dtype_code(pool_k.dtype)
-        _like("kv_commit_path", dev, pool_k=(pool_k, pool_k.dtype, None), pool_v=(pool_v, pool_k.dtype, pool_k.shape))
+        code, ks, vs = L.dtype_code(pool_k.dtype), None, None
+        _dense("kv_commit_path", dev, (pool_k, pool_k.dtype), (pool_v, pool_k.dtype), (block_tables, _I32), (start_lens, _I32),
+               (path, _I32), (n_accepted, _I32))
+        if pool_v.shape != pool_k.shape:
+            _refuse("kv_commit_path", f"caches of different shapes: {list(pool_k.shape)}, {list(pool_v.shape)}")
     else:
-        code = L.KVE_FP8_E4M3
         if k_scale is None or v_scale is None:
-            raise ValueError("kv_commit_path: k_scale and v_scale go together")
+            _refuse("kv_commit_path", "k_scale and v_scale go together")
+        code, ks, vs = L.KVE_FP8_E4M3, k_scale.data_ptr(), v_scale.data_ptr()
         _fp8_cache("kv_commit_path", dev, pool_k, pool_v, k_scale, v_scale)
-    _like("kv_commit_path", dev, block_tables=(block_tables, i32, None), start_lens=(start_lens, i32, None),
-          path=(path, i32, None), n_accepted=(n_accepted, i32, (B,)))
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or path.dim() != 2 or path.shape[0] != B:
-        raise ValueError("kv_commit_path: one block table row and one path row per sequence")
-    _call(lib.kve_kv_commit_path, dev, pool_k.data_ptr(), pool_v.data_ptr(), code, L.ptr(k_scale), L.ptr(v_scale), layers,
-          num_blocks, bs, nkv, hd, block_tables.data_ptr(), block_tables.shape[1], start_lens.data_ptr(), path.data_ptr(),
-          path.shape[1], n_accepted.data_ptr(), B, L.ptr(status))
+        _dense("kv_commit_path", dev, (block_tables, _I32), (start_lens, _I32), (path, _I32), (n_accepted, _I32))
+    if path_rows != B or start_lens.numel() != B or n_accepted.numel() != B:
+        _refuse("kv_commit_path", "one block table row, path row, start and count per sequence")
+    _call(lib.kve_kv_commit_path, dev, pool_k.data_ptr(), pool_v.data_ptr(), code, ks, vs, layers, num_blocks, bs, nkv, hd,
+          block_tables.data_ptr(), width, start_lens.data_ptr(), path.data_ptr(), path_width, n_accepted.data_ptr(), B,
+          L.ptr(status))
