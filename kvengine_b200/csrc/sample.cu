@@ -15,19 +15,20 @@
 // p where no w is positive).
 //
 // Two kernels. The first reads every logit once and leaves, per row and part of the
-// row, the maximum m and the sum of e^((x - m) / T) (T <= 0: the argmax instead):
+// row, the sum of e^(x / T) and the largest term it is relative to (T <= 0: the argmax):
 // HBM is its bound. The second runs a cluster of CTAs per sequence: each joins
 // the parts' sums of the rows it needs, walks the drafts (every CTA of the cluster
 // by itself: a few values) and scans its share of the one row the last token comes
 // from, which is often still in L2; the shares' best tokens meet through distributed
 // shared memory.
 //
-// Precision: x - m is taken before it is multiplied by 1 / T, so that large logits
-// lose nothing; e^x runs on ex2.approx (2^-22) into fp32 sums of a part's
-// thirty-odd values per thread, then pairwise. Acceptance, log-probabilities and
-// every thread's best candidate are recomputed in 64 bits from m and the sums, so
-// a token changes only where two candidates of one thread lie within fp32
-// rounding of each other. A NaN logit counts as minus infinity (never drawn).
+// Precision: a row is held as (b, z), z = sum 2^(x c - b) with c = log2(e) / T and
+// b the largest x c as rounded, so that every x c - b is one fused operation
+// rounded relative to itself, whatever the logits' size. 2^x runs on ex2.approx (2^-22)
+// into fp32 sums of a part's few dozen values per thread, then pairwise.
+// Acceptance, log-probabilities and the candidates within fp32 rounding of a CTA's
+// best are recomputed in 64 bits. A NaN logit counts as minus infinity (never drawn);
+// rows with one are summed again, slowly.
 #include <math.h>
 
 #include "kve_common.cuh"
@@ -35,8 +36,9 @@
 namespace kve {
 namespace {
 
-constexpr int kStatThreads = 512;
-constexpr int kDrawThreads = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kStatThreads = 256;
+constexpr int kDrawThreads = 256;  // and three CTAs a SM: 128 sequences' clusters run in one wave
 constexpr int kMaxParts = 32;     // parts of a row in the first kernel
 constexpr int kMaxNodes = 1024;   // nodes of a tree
 constexpr int kMaxK = 31;         // drafts of a chain
@@ -50,6 +52,9 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // NaN as minus infinity.
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 template <typename T> struct Pack;
 template <> struct Pack<float> {
@@ -101,10 +106,10 @@ __device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch
   for (int j = head + nvec * N + threadIdx.x; j < hi; j += THREADS) one(Elem<T>::to_f(row[j]), j);
 }
 
-// What the first kernel leaves of one part of a row. z: the sum of e^((x - m) / T),
-// or, for T <= 0, the column of the maximum.
+// What the first kernel leaves of one part of a row: its base and its sum, or, for
+// T <= 0, its largest logit and that one's column.
 struct Part {
-  float m, z;
+  float b, z;
 };
 
 // Where the rows of the first kernel lie: rows [0, n_first) at `first`, the others
@@ -138,7 +143,7 @@ __device__ __forceinline__ const T* row_at(const Rows& r, int row) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kStatThreads, 3)
+__global__ void __launch_bounds__(kStatThreads, 4)
 row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temperature, Part* out) {
   grid_dep_wait();
   grid_dep_launch();
@@ -177,103 +182,119 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
     }
     return;
   }
-  const float c = 1.4426950408889634f / t;
-  float m = -INFINITY, z = 0.f;
+  const float c = kLog2e / t;
+  float base = -INFINITY, z = 0.f;  // this thread's b and z
   auto rebase = [&](float top) {
-    if (top > m) {
-      z *= m == -INFINITY ? 0.f : ex2((m - top) * c);
-      m = top;
+    top *= c;
+    if (top > base) {
+      z *= ex2(base - top);  // 0 at the first
+      base = top;
     }
   };
   auto one = [&](float v, int) {
-    v = clean(v);
     rebase(v);
-    if (m != -INFINITY) z += v == m ? 1.f : ex2((v - m) * c);
+    z += ex2(fmaf(v, c, base == -INFINITY ? 0.f : -base));
   };
   auto batch = [&](auto& v, int) {
     constexpr int N = Pack<T>::N;
-    float top = v[0] = clean(v[0]);
+    float top = v[0];
 #pragma unroll
-    for (int j = 1; j < N; ++j) top = fmaxf(top, v[j] = clean(v[j]));
+    for (int j = 1; j < N; ++j) top = fmaxf(top, v[j]);  // passes over NaN
     rebase(top);
-    const float base = m == -INFINITY ? 0.f : m;
+    const float off = base == -INFINITY ? 0.f : -base;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = ex2((v[j] - base) * c);
+    for (int j = 0; j < N; ++j) v[j] = ex2(fmaf(v[j], c, off));
 #pragma unroll
     for (int w = N / 2; w > 0; w >>= 1)
 #pragma unroll
       for (int j = 0; j < w; ++j) v[j] += v[j + w];
     z += v[0];
   };
-  scan<T, kStatThreads, 4>(x, lo, hi, batch, one);
-  float top = m;
+  scan<T, kStatThreads, 8>(x, lo, hi, batch, one);
+  // the part's base, then its sum
+  auto block_max = [&](float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) sm[warp] = top;
-  __syncthreads();
-  top = sm[0];
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (lane == 0) sm[warp] = v;
+    __syncthreads();
+    v = sm[lane % (kStatThreads / 32)];
 #pragma unroll
-  for (int w = 1; w < kStatThreads / 32; ++w) top = fmaxf(top, sm[w]);
-  if (top == INFINITY) {
-    // infinite logits share the whole probability: count them
+    for (int o = kStatThreads / 64; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  float top = block_max(base);
+  bool odd = __syncthreads_or(!(z < INFINITY));  // a NaN, or infinite logits
+  if (odd) {
+    // infinite logits share the whole probability, NaN has none
+    base = -INFINITY;
+    for (int i = lo + threadIdx.x; i < hi; i += kStatThreads) base = fmaxf(base, Elem<T>::to_f(x[i]) * c);
+    top = block_max(base);
     z = 0.f;
-    for (int i = lo + threadIdx.x; i < hi; i += kStatThreads) z += Elem<T>::to_f(x[i]) == INFINITY ? 1.f : 0.f;
+    for (int i = lo + threadIdx.x; i < hi; i += kStatThreads) {
+      const float v = clean(Elem<T>::to_f(x[i]));
+      if (v != -INFINITY) z += top == INFINITY ? (v == INFINITY ? 1.f : 0.f) : ex2(fmaf(v, c, -top));
+    }
   } else {
-    z = m == -INFINITY ? 0.f : z * ex2((m - top) * c);
+    z = base == -INFINITY ? 0.f : z * ex2(base - top);
   }
   z = warp_sum(z);
   if (lane == 0) sz[warp] = z;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    float sum = 0.f;
-    for (int w = 0; w < kStatThreads / 32; ++w) sum += sz[w];
-    out[(size_t)row * parts + part] = Part{top, sum};
+  if (warp == 0) {
+    z = lane < kStatThreads / 32 ? sz[lane] : 0.f;
+    z = warp_sum(z);
+    if (lane == 0) out[(size_t)row * parts + part] = Part{top, z};
   }
 }
 
-// A row's parts joined by the 32 lanes of a warp (parts <= 32).
+// A row's parts joined.
 struct Row {
-  float m;    // the largest logit
-  double z;   // the sum of e^((x - m) / T)
+  double z;   // the sum of 2^(x c - b)
+  float b;    // the base (T <= 0: the largest logit)
   int arg;    // T <= 0: the column of the largest
 };
-__device__ __forceinline__ Row join(const Part* parts, int n, float t) {
-  const int lane = threadIdx.x & 31;
-  Part p{-INFINITY, 0.f};
-  if (lane < n) {
-    const float2 v = __ldcg(reinterpret_cast<const float2*>(parts) + lane);
-    p = Part{v.x, v.y};
+// Rows row_of(0) .. row_of(n - 1) into out, by all threads: `group` (a power of two of at
+// least n_parts) lanes a row.
+template <typename F>
+__device__ __forceinline__ void join_rows(const Part* parts, int n_parts, int group, float t, Row* out, int n, F&& row_of) {
+  const int sub = threadIdx.x & (group - 1), per = kDrawThreads / group;
+  for (int i0 = 0; i0 < n; i0 += per) {
+    const int i = i0 + threadIdx.x / group;
+    Part p{-INFINITY, 0.f};
+    if (i < n && sub < n_parts) {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(parts) + (size_t)row_of(i) * n_parts + sub);
+      p = Part{v.x, v.y};
+    }
+    float b = p.b;
+    for (int o = 1; o < group; o <<= 1) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+    Row r{1.0, b, 0x7fffffff};
+    if (!(t > 0.f)) {
+      r.arg = sub < n_parts && p.b == b ? __float_as_int(p.z) : 0x7fffffff;
+      for (int o = 1; o < group; o <<= 1) r.arg = min(r.arg, __shfl_xor_sync(0xffffffffu, r.arg, o));
+    } else {
+      r.z = p.b == -INFINITY ? 0.0 : p.b == b ? (double)p.z : (double)p.z * exp2((double)p.b - b);
+      for (int o = 1; o < group; o <<= 1) r.z += __shfl_xor_sync(0xffffffffu, r.z, o);
+    }
+    if (i < n && sub == 0) out[i] = r;
   }
-  float m = p.m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (!(t > 0.f)) {
-    int at = lane < n && p.m == m ? __float_as_int(p.z) : 0x7fffffff;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-    return Row{m, 1.0, at};
-  }
-  double z = lane < n && p.m != -INFINITY ? (p.m == m ? (double)p.z : (double)p.z * exp(((double)p.m - m) / t)) : 0.0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-  return Row{m, z, 0};
 }
-// (x - m) / T, and p of logit x at column v, in 64 bits.
-__device__ __forceinline__ double exponent(float x, float m, float t) { return x == m ? 0.0 : ((double)x - m) / t; }
+// log2 of e^(x / T) over e^(the base), and p of logit x at column v, in 64 bits.
+__device__ __forceinline__ double exponent(float x, float b, float t) {
+  return b == INFINITY ? (x == INFINITY ? 0.0 : -INFINITY) : (double)x * (double)(kLog2e / t) - b;
+}
 __device__ __forceinline__ double probability(const Row& r, float x, int v, float t) {
   if (!(t > 0.f)) return v == r.arg ? 1.0 : 0.0;
   x = clean(x);
   if (x == -INFINITY || !(r.z > 0.0)) return 0.0;
-  return exp(exponent(x, r.m, t)) / r.z;
+  return exp2(exponent(x, r.b, t)) / r.z;
 }
-
 struct DrawParams {
   const void* logits;       // target rows
   int64_t stride;
   const void* draft;        // chain: draft rows, or null
   int64_t dsb, dsj;
   const Part* parts;        // [rows][n_parts]: target rows, then draft rows
-  int n_parts;
+  int n_parts, group;
   const int32_t* drafts;    // chain: draft tokens (tree: node tokens)
   int64_t tsb, tsj;
   const int32_t* parents;   // tree
@@ -294,229 +315,308 @@ struct DrawParams {
   int* status;
 };
 
-// A candidate for the last token: its key in 64 bits and its column.
+// A candidate for the last token: its key in 64 bits, its column and its logit.
 struct Best {
   double key;
   int at;
+  float x;
 };
-__device__ __forceinline__ void take(Best& b, double key, int at) {
-  if (at >= 0 && (b.at < 0 || key > b.key || (key == b.key && at < b.at))) b = Best{key, at};
+__device__ __forceinline__ Best better(Best a, Best b) {
+  return b.at >= 0 && (a.at < 0 || b.key > a.key || (b.key == a.key && b.at < a.at)) ? b : a;
+}
+__device__ __forceinline__ Best warp_best(Best b) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    b = better(b, Best{__shfl_xor_sync(0xffffffffu, b.key, o), __shfl_xor_sync(0xffffffffu, b.at, o),
+                       __shfl_xor_sync(0xffffffffu, b.x, o)});
+  return b;
 }
 
-// The draw: best candidate of columns [lo, hi). `qrow` (may be null): subtract the
-// draft's distribution. `skip`: tokens that may not be drawn.
+// Shared memory of a draw.
+struct DrawShared {
+  Best kept[kDrawThreads];
+  Best share[8];               // rank 0's: the best of each CTA of the cluster
+  Best best;
+  float lz, inv_zp, inv_zq;    // log2 z of the target's row; 1 / z of it and of the draft's
+  int bar;                     // the CTA's best fp32 key so far, as an ordered integer
+  int n;                       // candidates kept
+};
+__device__ __forceinline__ int ordered(float f) {
+  const int i = __float_as_int(f);
+  return i < 0 ? i ^ 0x7fffffff : i;
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i < 0 ? i ^ 0x7fffffff : i); }
+
+// Keys (log2 of a weight, plus gumbel log2 e) in fp32 are good to a few 1e-6; what lies
+// this close below the best is looked at in 64 bits.
+constexpr float kMargin = 1e-4f;
+
+// The CTA's best candidate of columns [lo, hi), in every lane of warp 0. `qrow` (may be
+// null): the draft's row, whose distribution is subtracted. `skip`: tokens not to draw.
+//
+// A column's key is at most its key without the draft, so the scan compares that
+// with the CTA's best so far, and only the few columns that pass it cost an
+// exponential, a logarithm and a look at the draft's row.
 template <typename T>
-__device__ __forceinline__ Best draw_share(const T* row, const Row& p, const T* qrow, const Row& q, const float* gumbel,
-                                           float t, int lo, int hi, const int* skip, int n_skip) {
-  Best best{-INFINITY, -1};
+__device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, const T* row, const Row& p, const T* qrow,
+                                             const Row& q, const float* gumbel, float t, const int* skip, int n_skip) {
+  constexpr int N = Pack<T>::N;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();  // an earlier draw's values have been read
+  if (threadIdx.x == 0) {
+    sh.bar = ordered(-INFINITY);
+    sh.n = 0;
+    sh.lz = (float)log2(p.z);
+    sh.inv_zp = (float)(1.0 / p.z);
+  } else if (threadIdx.x == 32) {
+    sh.inv_zq = qrow && q.z > 0.0 ? (float)(1.0 / q.z) : 0.f;
+  }
+  // 16 bytes of logits at a time from their first 16-byte boundary on, and their noise
+  const int mis = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
+  const int head = min(lo + (mis ? N - mis : 0), hi);
+  const int nvec = (hi - head) / N;
+  const uint4* xv = reinterpret_cast<const uint4*>(row + head);
+  const float* gh = gumbel + head;
+  const bool even = (reinterpret_cast<uintptr_t>(gh) & 15) == 0;
+  auto noise = [&](int i, float* g) {
+    if (even) {
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(gh) + (size_t)i * (N / 4) + j);
+        g[4 * j] = f.x;
+        g[4 * j + 1] = f.y;
+        g[4 * j + 2] = f.z;
+        g[4 * j + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) g[j] = gh[(size_t)i * N + j];
+    }
+  };
   float key = -INFINITY;
   int at = -1;
-  const float inv = 1.f / t;
-  auto skipped = [&](int v) {
-    for (int j = 0; j < n_skip; ++j)
-      if (skip[j] == v) return true;
-    return false;
-  };
-  if (!(p.z > 0.0)) return best;
-  if (!qrow) {
-    auto one = [&](float x, int v) {
-      x = clean(x);
-      const float e = x == p.m ? 0.f : (x - p.m) * inv;
-      const float s = e + gumbel[v];
-      if (s > key && !skipped(v)) { key = s; at = v; }
-    };
-    auto batch = [&](auto& x, int v) {
-#pragma unroll
-      for (int j = 0; j < Pack<T>::N; ++j) one(x[j], v + j);
-    };
-    scan<T, kDrawThreads, 1>(row, lo, hi, batch, one);
-    if (at >= 0) best = Best{exponent(clean(Elem<T>::to_f(row[at])), p.m, t) + (double)gumbel[at], at};
-    return best;
-  }
-  const float c = 1.4426950408889634f * inv;
-  const float zp = (float)(1.0 / p.z), zq = q.z > 0.0 ? (float)(1.0 / q.z) : 0.f;
-  const float lzp = (float)log(p.z);
-  auto one = [&](float x, int v) {
-    x = clean(x);
-    const float e = x == p.m ? 0.f : x - p.m;
-    const float gv = gumbel[v];
-    // log(p - q) <= log p: most columns are out of the question without an exponential
-    if (!(e * inv - lzp + gv > key - 1e-4f)) return;
-    const float y = clean(Elem<T>::to_f(qrow[v]));
-    const float w = ex2(e * c) * zp - (y == q.m ? 1.f : ex2((y - q.m) * c)) * zq;
-    if (!(w > 0.f)) return;
-    const float s = __logf(w) + gv;
-    if (s > key) { key = s; at = v; }
-  };
-  auto batch = [&](auto& x, int v) {
-#pragma unroll
-    for (int j = 0; j < Pack<T>::N; ++j) one(x[j], v + j);
-  };
-  scan<T, kDrawThreads, 1>(row, lo, hi, batch, one);
-  if (at >= 0) {
-    const double w = probability(p, Elem<T>::to_f(row[at]), at, t) - probability(q, Elem<T>::to_f(qrow[at]), at, t);
-    best = Best{(w > 0.0 ? log(w) : (double)key - gumbel[at]) + (double)gumbel[at], at};
-  }
-  return best;
-}
-
-// The best of the whole cluster, in every CTA's thread 0 of rank 0.
-__device__ __forceinline__ Best join_shares(Best b, int shares, int rank) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const double ok = __shfl_xor_sync(0xffffffffu, b.key, o);
-    const int oa = __shfl_xor_sync(0xffffffffu, b.at, o);
-    take(b, ok, oa);
-  }
-  __shared__ double sk[kDrawThreads / 32];
-  __shared__ int sa[kDrawThreads / 32];
-  __shared__ double mine_key;
-  __shared__ int mine_at;
-  __syncthreads();  // a second draw: every thread has read the first one's result
-  if (lane == 0) { sk[warp] = b.key; sa[warp] = b.at; }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kDrawThreads / 32; ++w) take(b, sk[w], sa[w]);
-    mine_key = b.key;
-    mine_at = b.at;
-  }
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  // every CTA reads all shares, so that all agree on whether a second scan is needed
-  if (threadIdx.x == 0) {
-    const uint32_t ak = static_cast<uint32_t>(__cvta_generic_to_shared(&mine_key));
-    const uint32_t aa = static_cast<uint32_t>(__cvta_generic_to_shared(&mine_at));
-    for (int s = 0; s < shares; ++s) {
-      if (s == rank) continue;
-      uint32_t rk, ra;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(rk) : "r"(ak), "r"(s));
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(aa), "r"(s));
-      double ok;
-      int oa;
-      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(ok) : "r"(rk) : "memory");
-      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(oa) : "r"(ra) : "memory");
-      take(b, ok, oa);
+  if (p.z > 0.0) {
+    const float c = kLog2e / t, lz = sh.lz, off = p.b == INFINITY ? 0.f : -p.b;
+    auto weigh = [&](float x) { return p.b == INFINITY ? (x == INFINITY ? 0.f : -INFINITY) : fmaf(x, c, off); };
+    volatile int* bar = &sh.bar;
+    auto consider = [&](float e, float gv, int v) {  // e: log2 of the weight without the draft, times z
+      float k = e - lz + gv;
+      if (qrow) {
+        const float y = clean(Elem<T>::to_f(qrow[v]));
+        const float qw = q.b == INFINITY ? (y == INFINITY ? 1.f : 0.f) : ex2(fmaf(y, c, -q.b));
+        const float w = ex2(e) * sh.inv_zp - qw * sh.inv_zq;
+        k = w > 0.f ? __log2f(w) + gv : -INFINITY;
+      }
+      if (!(k > key)) return;
+      for (int j = 0; j < n_skip; ++j)
+        if (skip[j] == v) return;
+      key = k;
+      at = v;
+      if (ordered(k) > *bar) atomicMax(&sh.bar, ordered(k));
+    };
+    auto one = [&](float x, int v) {
+      const float e = weigh(clean(x)), gv = gumbel[v] * kLog2e;
+      if (e - lz + gv > unordered(*bar) - kMargin) consider(e, gv, v);
+    };
+    auto batch = [&](const float* x, const float* g, int v) {
+      float top = -INFINITY;
+      float e[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        e[j] = weigh(x[j]);
+        top = fmaxf(top, fmaf(g[j], kLog2e, e[j]));
+      }
+      if (!(top - lz > unordered(*bar) - kMargin)) return;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (fmaf(g[j], kLog2e, e[j]) - lz > unordered(*bar) - kMargin) consider(e[j], g[j] * kLog2e, v + j);
+    };
+    for (int i = lo + threadIdx.x; i < head; i += kDrawThreads) one(Elem<T>::to_f(row[i]), i);
+    constexpr int U = sizeof(T) == 4 ? 4 : 2;
+    for (int i0 = threadIdx.x; i0 < nvec; i0 += U * kDrawThreads) {
+      uint4 raw[U];
+      float g[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * kDrawThreads < nvec) {
+          raw[u] = __ldcg(xv + i0 + u * kDrawThreads);
+          noise(i0 + u * kDrawThreads, g[u]);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * kDrawThreads < nvec) {
+          float x[N];
+          Pack<T>::unpack(raw[u], x);
+          batch(x, g[u], head + (i0 + u * kDrawThreads) * N);
+        }
     }
-    sk[0] = b.key;
-    sa[0] = b.at;
+    for (int j = head + nvec * N + threadIdx.x; j < hi; j += kDrawThreads) one(Elem<T>::to_f(row[j]), j);
   }
-  // nobody leaves, or writes its share again, before all have read it
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  return Best{sk[0], sa[0]};
+  __syncthreads();
+  if (at >= 0 && key >= unordered(sh.bar) - kMargin) {
+    const float x = clean(Elem<T>::to_f(row[at]));
+    const double gv = gumbel[at];
+    double k = key * 0.6931471805599453;  // stands where the weight rounds to nothing in 64 bits
+    if (qrow) {
+      const double w = probability(p, x, at, t) - probability(q, Elem<T>::to_f(qrow[at]), at, t);
+      if (w > 0.0) k = log(w) + gv;
+    } else {
+      k = (p.b == INFINITY ? 0.0 : (double)x / t) + gv;
+    }
+    sh.kept[atomicAdd(&sh.n, 1)] = Best{k, at, x};
+  }
+  __syncthreads();
+  Best b{-INFINITY, -1, 0.f};
+  if (warp == 0) {
+    for (int i = lane; i < sh.n; i += 32) b = better(b, sh.kept[i]);
+    b = warp_best(b);
+  }
+  return b;
 }
 
-// Scan, and where nothing may be drawn (every weight zero), scan again for p itself.
+// The token drawn by the cluster, in rank 0 (the others' result means nothing; they
+// are done). Where no weight is positive, rank 0 draws from p alone.
 template <typename T>
-__device__ __forceinline__ int draw(const DrawParams& a, const T* row, const Row& p, const T* qrow, const Row& q,
-                                    const float* gumbel, float t, int rank, const int* skip, int n_skip) {
+__device__ __forceinline__ Best draw(const DrawParams& a, DrawShared& sh, const T* row, const Row& p, const T* qrow,
+                                     const Row& q, const float* gumbel, float t, int rank, const int* skip, int n_skip) {
   const int lo = min(rank * a.chunk, a.vocab), hi = min(a.vocab, lo + a.chunk);
-  const Row none{0.f, 0.0, 0};
-  Best b = join_shares(draw_share<T>(row, p, qrow, q, gumbel, t, lo, hi, skip, n_skip), a.shares, rank);
-  if (b.at < 0 && (qrow || n_skip))
-    b = join_shares(draw_share<T>(row, p, nullptr, none, gumbel, t, lo, hi, skip, 0), a.shares, rank);
-  return b.at < 0 ? 0 : b.at;
+  const int lane = threadIdx.x & 31;
+  Best b = draw_columns<T>(sh, lo, hi, row, p, qrow, q, gumbel, t, skip, n_skip);
+  cluster_wait();  // every CTA of the cluster has started: rank 0's memory is there
+  if (threadIdx.x == 0) {
+    uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.share[rank]));
+    asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(to) : "r"(0));
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(b.key) : "memory");
+    asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(to + 8), "r"(b.at), "r"(__float_as_int(b.x)) : "memory");
+  }
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (rank != 0) return b;
+  if (threadIdx.x < 32) {
+    b = Best{-INFINITY, -1, 0.f};
+    if (lane < a.shares) b = sh.share[lane];
+    b = warp_best(b);
+    if (lane == 0) sh.best = b;
+  }
+  __syncthreads();
+  b = sh.best;
+  if (b.at < 0 && (qrow || n_skip)) {
+    b = draw_columns<T>(sh, 0, a.vocab, row, p, nullptr, p, gumbel, t, skip, 0);
+    if (threadIdx.x == 0) sh.best = b;
+    __syncthreads();
+    b = sh.best;
+  }
+  if (b.at < 0) b = Best{0.0, 0, -INFINITY};  // no probability anywhere
+  return b;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kDrawThreads)
+__global__ void __launch_bounds__(kDrawThreads, 3)
 chain_draw_kernel(DrawParams a) {
+  cluster_arrive();
   grid_dep_wait();
   grid_dep_launch();
   const int b = blockIdx.x / a.shares, rank = blockIdx.x % a.shares;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int k = a.k;
+  const int k = a.k, tid = threadIdx.x;
   const float t = a.temperature[b];
   const T* logits = static_cast<const T*>(a.logits) + (int64_t)b * (k + 1) * a.stride;
   const T* draft = a.draft ? static_cast<const T*>(a.draft) + b * a.dsb : nullptr;
-  __shared__ Row prow[kMaxK + 1], qrow[kMaxK];
-  __shared__ double pd[kMaxK], qd[kMaxK];
+  __shared__ Row rows[2 * kMaxK + 1];  // target rows 0 .. k, then draft rows
+  __shared__ double pd[kMaxK];         // p of the drafts
   __shared__ int tok[kMaxK];
   __shared__ int n_s;
-  for (int r = warp; r < 2 * k + 1; r += kDrawThreads / 32) {
-    if (r > k && !draft) break;
-    const int row = r <= k ? b * (k + 1) + r : a.batch * (k + 1) + b * k + (r - k - 1);
-    const Row x = join(a.parts + (size_t)row * a.n_parts, a.n_parts, t);
-    if (lane != 0) continue;
-    const int j = r <= k ? r : r - k - 1;
-    (r <= k ? prow : qrow)[j] = x;
-    if (j == k) continue;
-    const int d = a.drafts[b * a.tsb + j * a.tsj];
-    const bool ok = d >= 0 && d < a.vocab;
-    const double pr = !ok ? 0.0 : probability(x, Elem<T>::to_f((r <= k ? logits + j * a.stride : draft + j * a.dsj)[d]), d, t);
-    (r <= k ? pd : qd)[j] = pr;
-    if (r <= k) {
-      if (!ok && rank == 0) report(a.status, KVE_ERR_BOUNDS);
-      tok[j] = ok ? d : -1;
-      if (!draft) qd[j] = 1.0;
+  __shared__ DrawShared sh;
+  // Thread j fetches draft j and its logits while the rows' sums are joined.
+  int d = -1;
+  float x = 0.f, y = 0.f, u = 0.f;
+  if (tid < k) {
+    d = a.drafts[b * a.tsb + tid * a.tsj];
+    u = a.u[b * a.usb + tid];
+    if (d < 0 || d >= a.vocab) {
+      if (rank == 0) report(a.status, KVE_ERR_BOUNDS);
+      d = -1;
+    } else {
+      x = Elem<T>::to_f(logits[tid * a.stride + d]);
+      if (draft) y = Elem<T>::to_f(draft[tid * a.dsj + d]);
     }
+    tok[tid] = d;
   }
+  join_rows(a.parts, a.n_parts, a.group, t, rows, draft ? 2 * k + 1 : k + 1,
+            [&](int i) { return i <= k ? b * (k + 1) + i : a.batch * (k + 1) + b * k + (i - k - 1); });
   __syncthreads();
-  if (warp == 0) {
-    const bool no = lane < k && !(tok[lane] >= 0 && (double)a.u[b * a.usb + lane] * qd[lane] < pd[lane]);
+  if (tid < 32) {
+    bool no = false;
+    if (tid < k) {
+      const double p = d < 0 ? 0.0 : probability(rows[tid], x, d, t);
+      const double q = d < 0 || !draft ? 1.0 : probability(rows[k + 1 + tid], y, d, t);
+      pd[tid] = p;
+      no = !((double)u * q < p);
+    }
     const unsigned m = __ballot_sync(0xffffffffu, no);
-    if (lane == 0) n_s = m ? __ffs(m) - 1 : k;
+    if (tid == 0) n_s = m ? __ffs(m) - 1 : k;
   }
   __syncthreads();
   const int n = n_s;
-  const T* row = logits + n * a.stride;
-  const float* gumbel = a.gumbel + b * a.gstride;
-  const Row p = prow[n];
-  int last;
+  const Row p = rows[n];
+  Best last;
   if (!(t > 0.f)) {
-    last = p.arg;  // one-hot: a rejected draft was another token
-    if (last < 0 || last >= a.vocab) last = 0;
+    cluster_wait();
+    last = Best{0.0, p.arg < a.vocab ? p.arg : 0, 0.f};  // one-hot: a rejected draft was another token
   } else {
     const bool sub = draft && n < k;
-    last = draw<T>(a, row, p, sub ? draft + n * a.dsj : nullptr, sub ? qrow[n] : p, gumbel, t, rank, tok + n,
-                   !draft && n < k ? 1 : 0);
+    last = draw<T>(a, sh, logits + n * a.stride, p, sub ? draft + n * a.dsj : nullptr, sub ? rows[k + 1 + n] : p,
+                   a.gumbel + b * a.gstride, t, rank, tok + n, !draft && n < k ? 1 : 0);
   }
-  if (rank != 0 || warp != 0) return;
-  if (lane <= k) {
-    const int e = lane < n ? tok[lane] : lane == n ? last : -1;
-    float lp = 0.f;
-    if (lane <= n && t > 0.f) {
-      const Row& r = prow[lane];
-      const float x = clean(Elem<T>::to_f(logits[lane * a.stride + e]));
-      lp = r.z > 0.0 && x != -INFINITY ? (float)(exponent(x, r.m, t) - log(r.z)) : -INFINITY;
-    }
-    a.emitted[(size_t)b * a.width + lane] = e;
-    a.logp[(size_t)b * a.width + lane] = lp;
-  }
-  if (lane == 0) a.n_acc[b] = n;
+  if (rank != 0 || tid > k) return;
+  float lp = 0.f;
+  if (t > 0.f && tid <= n) lp = (float)log(tid < n ? pd[tid] : probability(p, last.x, last.at, t));
+  a.emitted[(size_t)b * a.width + tid] = tid < n ? tok[tid] : tid == n ? last.at : -1;
+  a.logp[(size_t)b * a.width + tid] = lp;
+  if (tid == 0) a.n_acc[b] = n;
 }
 
-// Dynamic shared memory of the tree: per node its token, parent, p at its parent,
-// random number; then the path and the rejected tokens of its last node.
-constexpr size_t tree_smem(int nodes) { return (size_t)nodes * (sizeof(double) + 3 * sizeof(int) + 2 * sizeof(int)); }
+// Dynamic shared memory of a tree: per node its row, p of its token at its parent
+// (before: that logit), token, parent, random number, first accepted child; the path;
+// the tokens rejected at its end.
+constexpr size_t tree_smem(int nodes) { return (size_t)nodes * (sizeof(Row) + sizeof(double) + 6 * sizeof(int)); }
 
 template <typename T>
-__global__ void __launch_bounds__(kDrawThreads)
+__global__ void __launch_bounds__(kDrawThreads, 3)
 tree_draw_kernel(DrawParams a) {
+  cluster_arrive();
   grid_dep_wait();
   grid_dep_launch();
   extern __shared__ __align__(16) uint8_t dyn[];
   const int b = blockIdx.x / a.shares, rank = blockIdx.x % a.shares;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x;
   const int n = a.q_lens[b], off = a.q_offsets[b];
   const float t = a.temperature[b];
   // every CTA of the cluster sees the same values: all leave or none
   if (n < 1 || n > a.max_nodes || off < 0 || off > a.n_rows - n) {
-    if (threadIdx.x == 0 && rank == 0) {
+    if (tid == 0 && rank == 0) {
       if (n != 0) report(a.status, KVE_ERR_BOUNDS);
       a.n_acc[b] = -1;
     }
+    cluster_wait();
     return;
   }
-  double* pt = reinterpret_cast<double*>(dyn);
+  Row* rows = reinterpret_cast<Row*>(dyn);
+  double* pt = reinterpret_cast<double*>(rows + a.max_nodes);
   int* tok = reinterpret_cast<int*>(pt + a.max_nodes);
   int* par = tok + a.max_nodes;
   float* us = reinterpret_cast<float*>(par + a.max_nodes);
-  int* path = reinterpret_cast<int*>(us + a.max_nodes);
+  int* next = reinterpret_cast<int*>(us + a.max_nodes);
+  int* path = next + a.max_nodes;
   int* skip = path + a.max_nodes;
   __shared__ int s_n, s_skip;
+  __shared__ DrawShared sh;
   const T* logits = static_cast<const T*>(a.logits) + (int64_t)off * a.stride;
-  for (int i = threadIdx.x; i < n; i += kDrawThreads) {
+  if (tid == 0) s_skip = 0;
+  for (int i = tid; i < n; i += kDrawThreads) {
     int d = a.drafts[off + i], pa = a.parents[off + i];
+    us[i] = a.u[off + i];
     if (i == 0) pa = -1;
     else if (pa < 0 || pa >= i || d < 0 || d >= a.vocab) {
       if (rank == 0) report(a.status, KVE_ERR_BOUNDS);
@@ -524,66 +624,59 @@ tree_draw_kernel(DrawParams a) {
     }
     tok[i] = d;
     par[i] = pa;
-    us[i] = a.u[off + i];
+    next[i] = 0x7fffffff;
+    pt[i] = pa < 0 ? 0.0 : (double)Elem<T>::to_f(logits[pa * a.stride + d]);
   }
+  join_rows(a.parts, a.n_parts, a.group, t, rows, n, [&](int i) { return off + i; });
   __syncthreads();
-  // p of every node's token at its parent (0 for a token an earlier sibling has too).
-  for (int i = warp; i < n; i += kDrawThreads / 32) {
+  // p of every node's token at its parent: 0 for a token an earlier sibling has too
+  for (int i = tid; i < n; i += kDrawThreads) {
     const int pa = par[i];
     if (pa < 0) continue;
     bool twice = false;
-    for (int j = pa + 1 + lane; j < i; j += 32) twice |= par[j] == pa && tok[j] == tok[i];
-    twice = __any_sync(0xffffffffu, twice);
-    const Row r = join(a.parts + (size_t)(off + pa) * a.n_parts, a.n_parts, t);
-    if (lane == 0) pt[i] = twice ? 0.0 : probability(r, Elem<T>::to_f(logits[pa * a.stride + tok[i]]), tok[i], t);
+    for (int j = pa + 1; j < i; ++j) twice |= par[j] == pa && tok[j] == tok[i];
+    pt[i] = twice ? 0.0 : probability(rows[pa], (float)pt[i], tok[i], t);
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int cur = 0, m = 0, rejected = 0;
+  // what a node's earlier siblings leave, should all be rejected; its parent's first accepted child
+  for (int i = tid; i < n; i += kDrawThreads) {
+    const int pa = par[i];
+    if (pa < 0) continue;
     double left = 1.0;
-    path[0] = 0;
-    for (int i = 1; i < n; ++i) {
-      if (par[i] != cur) continue;
-      if ((double)us[i] * left < pt[i]) {
-        cur = i;
-        path[++m] = i;
-        left = 1.0;
-        rejected = 0;
-      } else {
-        left -= pt[i];
-        skip[rejected++] = tok[i];
-      }
-    }
-    s_n = m;
-    s_skip = rejected;
+    for (int j = pa + 1; j < i; ++j)
+      if (par[j] == pa) left -= pt[j];
+    if ((double)us[i] * left < pt[i]) atomicMin(&next[pa], i);
   }
   __syncthreads();
-  const int m = s_n;
-  const int node = path[m];
-  const Row p = join(a.parts + (size_t)(off + node) * a.n_parts, a.n_parts, t);
-  int last;
+  if (tid == 0) {
+    int m = 0;
+    path[0] = 0;
+    for (int i = next[0]; i < n; i = next[i]) path[++m] = i;
+    s_n = m;
+  }
+  __syncthreads();
+  const int m = s_n, node = path[m];
+  for (int i = node + 1 + tid; i < n; i += kDrawThreads)
+    if (par[i] == node) skip[atomicAdd(&s_skip, 1)] = tok[i];
+  __syncthreads();
+  const Row p = rows[node];
+  Best last;
   if (!(t > 0.f)) {
-    last = p.arg;
-    if (last < 0 || last >= a.vocab) last = 0;
+    cluster_wait();
+    last = Best{0.0, p.arg < a.vocab ? p.arg : 0, 0.f};
   } else {
-    last = draw<T>(a, logits + node * a.stride, p, nullptr, p, a.gumbel + b * a.gstride, t, rank, skip, s_skip);
+    last = draw<T>(a, sh, logits + node * a.stride, p, static_cast<const T*>(nullptr), p, a.gumbel + b * a.gstride, t, rank,
+                   skip, s_skip);
   }
   if (rank != 0) return;
-  for (int j = warp; j < a.width; j += kDrawThreads / 32) {
-    const int at = j <= m ? path[j] : -1;
-    const int e = j < m ? tok[path[j + 1]] : j == m ? last : -1;
-    float lp = 0.f;
-    if (j <= m && t > 0.f) {
-      const Row r = join(a.parts + (size_t)(off + at) * a.n_parts, a.n_parts, t);
-      const float x = clean(Elem<T>::to_f(logits[at * a.stride + e]));
-      lp = r.z > 0.0 && x != -INFINITY ? (float)(exponent(x, r.m, t) - log(r.z)) : -INFINITY;
-    }
-    if (lane != 0) continue;
-    a.path[(size_t)b * a.width + j] = at;
-    a.emitted[(size_t)b * a.width + j] = e;
-    a.logp[(size_t)b * a.width + j] = lp;
+  for (int j = tid; j < a.width; j += kDrawThreads) {
+    const size_t to = (size_t)b * a.width + j;
+    const int child = j < m ? path[j + 1] : -1;
+    a.path[to] = j <= m ? path[j] : -1;
+    a.emitted[to] = j < m ? tok[child] : j == m ? last.at : -1;
+    a.logp[to] = t > 0.f && j <= m ? (float)log(j < m ? pt[child] : probability(p, last.x, last.at, t)) : 0.f;
   }
-  if (threadIdx.x == 0) a.n_acc[b] = m;
+  if (tid == 0) a.n_acc[b] = m;
 }
 
 // ------------------------------------------------------------------ host
@@ -593,11 +686,16 @@ int stat_parts(int rows, int vocab) {
   const int most = vocab / 4096 < kMaxParts ? vocab / 4096 : kMaxParts;
   return want < most ? want : most < 1 ? 1 : most;
 }
-// CTAs of a sequence's cluster in the second kernel.
+// CTAs of a sequence's cluster in the second kernel: at most one wave of them.
 int draw_shares(int batch, int vocab) {
   const int want = 3 * 148 / batch, most = vocab / 4096;
   const int n = want < most ? want : most;
-  return n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
+  return n > 8 ? 8 : n < 1 ? 1 : n;
+}
+int lanes_for(int parts) {
+  int n = 1;
+  while (n < parts) n *= 2;
+  return n;
 }
 int round_up(int n, int to) { return (n + to - 1) / to * to; }
 size_t workspace_of(int64_t rows, int vocab) {
@@ -613,6 +711,13 @@ int run_stats(const char* me, const Rows& rows, int n_rows, int vocab, const flo
 }
 template <typename Kernel>
 int run_draw(const char* me, Kernel kernel, const DrawParams& a, size_t smem, cudaStream_t stream) {
+  if (smem > 32768) {  // with the static part, more than a kernel has without asking
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(KVE_ERR_CUDA, "%s: %s", me, cudaGetErrorString(err));
+    }
+  }
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = a.shares;
@@ -666,7 +771,7 @@ extern "C" int kve_sample_accept(const void* logits, int dtype, int64_t row_stri
   if (rc) return rc;
   DrawParams a{};
   a.logits = logits; a.stride = row_stride; a.draft = draft_logits; a.dsb = draft_logits_stride_b; a.dsj = draft_logits_stride_j;
-  a.parts = parts; a.n_parts = n_parts; a.drafts = drafts; a.tsb = draft_stride_b; a.tsj = draft_stride_j;
+  a.parts = parts; a.n_parts = n_parts; a.group = lanes_for(n_parts); a.drafts = drafts; a.tsb = draft_stride_b; a.tsj = draft_stride_j;
   a.u = uniforms; a.usb = uniform_stride_b; a.gumbel = gumbel; a.gstride = gumbel_stride; a.temperature = temperature;
   a.batch = batch; a.k = k; a.vocab = vocab; a.shares = draw_shares(batch, vocab);
   a.chunk = round_up((vocab + a.shares - 1) / a.shares, 8);
@@ -705,7 +810,7 @@ extern "C" int kve_tree_sample_accept(const void* logits, int dtype, int64_t row
                             : run_stats<__nv_bfloat16>(me, rows, n_rows, vocab, temperature, parts, n_parts, stream);
   if (rc) return rc;
   DrawParams a{};
-  a.logits = logits; a.stride = row_stride; a.parts = parts; a.n_parts = n_parts; a.drafts = tokens; a.parents = parents;
+  a.logits = logits; a.stride = row_stride; a.parts = parts; a.n_parts = n_parts; a.group = lanes_for(n_parts); a.drafts = tokens; a.parents = parents;
   a.q_lens = q_lens; a.q_offsets = q_offsets; a.u = uniforms; a.gumbel = gumbel; a.gstride = gumbel_stride;
   a.temperature = temperature; a.batch = batch; a.vocab = vocab; a.n_rows = n_rows; a.max_nodes = max_q_len;
   a.shares = draw_shares(batch, vocab); a.chunk = round_up((vocab + a.shares - 1) / a.shares, 8);
