@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "kve_common.cuh"
+#include "tree_attn.cuh"
 
 namespace kve {
 namespace {
@@ -45,43 +46,11 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;       // keys per tile
 constexpr int kMaxGroup = 64;
 constexpr int kMaxNodes = 1024;
-// The workspace starts with the arrival counters, at the same addresses for every
-// call and every op that shares it, so that no call's partials ever land on them.
-constexpr size_t kCounterSlots = 16384;
-constexpr size_t kCounterBytes = kCounterSlots * sizeof(int32_t);
 
 enum { kBf16 = 0, kFp8 = 1, kF32 = 2 };
 
-struct TreeParams {
-  const void* q;
-  const void* pool_k;
-  const void* pool_v;
-  const uint8_t* k_scale;
-  const uint8_t* v_scale;
-  const int32_t* tables;
-  int table_stride;
-  const int32_t* ctx_lens;
-  const int32_t* q_lens;
-  const int32_t* q_offsets;
-  const uint32_t* mask;
-  int mask_words;
-  int max_q, nq, nkv, group, bs;
-  int64_t num_blocks;
-  float scale;
-  void* out;
-  int* counters;
-  float* partials;
-  int chunk, n_chunks, n_qtiles;
-  int* status;
-};
-
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -209,17 +178,6 @@ __device__ __forceinline__ int swz(int key, int piece) {
   if constexpr (CH == 4) return piece ^ ((key >> 1) & 3);
   if constexpr (KV == kF32) return piece ^ ((key & 2) | (((key >> 2) ^ key) & 1) << 2);
   return piece ^ ((key & 1) << 2 | (key & 2) | (key >> 2 & 1));
-}
-
-// Bits j0 .. j0+15 of a row's mask, as seen from key j0 of the new tokens
-// (negative: history, always seen). Bits past the words are clear.
-__device__ __forceinline__ uint32_t mask_bits(const uint32_t* row, int words, int j0) {
-  const int lo = j0 < 0 ? 0 : j0;
-  const int w = lo >> 5, s = lo & 31;
-  uint32_t v = w < words ? row[w] >> s : 0u;
-  if (s && w + 1 < words) v |= row[w + 1] << (32 - s);
-  if (j0 < 0) v = v << -j0 | ((1u << -j0) - 1u);  // j0 > -16 here
-  return v;
 }
 
 template <int KV, int HD, int RB>
@@ -492,15 +450,8 @@ tree_attn_kernel(TreeParams p) {
     uint32_t see_lo = 0xffffu, see_hi = 0xffffu;
     if (masked) {
       const int j0 = kt - hist;
-      if (j0 > -kTile) {
-        if (p.mask) {
-          see_lo = mask_bits(mask_lo, p.mask_words, j0);
-          see_hi = mask_bits(mask_hi, p.mask_words, j0);
-        } else {  // key kt + x is seen where j0 + x <= node
-          see_lo = n_lo < j0 ? 0u : n_lo - j0 >= 31 ? ~0u : (2u << (n_lo - j0)) - 1u;
-          see_hi = n_hi < j0 ? 0u : n_hi - j0 >= 31 ? ~0u : (2u << (n_hi - j0)) - 1u;
-        }
-      }
+      see_lo = p.mask ? mask_bits<kTile>(mask_lo, p.mask_words, j0) : chain_bits(n_lo, j0);
+      see_hi = p.mask ? mask_bits<kTile>(mask_hi, p.mask_words, j0) : chain_bits(n_hi, j0);
       const uint32_t inside = key_hi - kt >= kTile ? 0xffffu : (1u << (key_hi - kt)) - 1u;
       see_lo &= inside;
       see_hi &= inside;
@@ -793,6 +744,10 @@ size_t partial_bytes(const Split& s, int batch, int nkv, int hd) {
   return (size_t)batch * nkv * s.n_qtiles * s.n_chunks * (s.rb * 16) * (hd + 4) * sizeof(float);
 }
 
+// The wide kernel's tile is 128 rows: it is for trees of more rows than this per kv head.
+constexpr int kWideRows = 32;
+bool use_wide(int max_q, int group) { return (long long)max_q * group > kWideRows; }
+
 template <int KV, int HD, int RB>
 int launch(const TreeParams& p, int batch, cudaStream_t stream) {
   // the shared-memory limit is an attribute of the kernel on one device
@@ -834,8 +789,12 @@ extern "C" size_t kve_tree_attn_workspace_bytes(int batch, int max_q_len, int ma
   if (batch < 1 || max_q_len < 1 || max_ctx < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1)
     return 0;
   const Split s = split_of(batch, max_q_len, max_ctx, num_kv_heads, num_heads / num_kv_heads);
-  const size_t n = partial_bytes(s, batch, num_kv_heads, head_dim);
-  return n ? kCounterBytes + n : 0;
+  size_t n = partial_bytes(s, batch, num_kv_heads, head_dim);
+  if (use_wide(max_q_len, num_heads / num_kv_heads)) {  // the call's types and block size choose the kernel
+    const size_t w = tree_attn_wide_partial_bytes(batch, max_q_len, max_ctx, num_kv_heads, num_heads / num_kv_heads, head_dim);
+    n = n > w ? n : w;
+  }
+  return n ? kTreeCounterBytes + n : 0;
 }
 
 extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k, const void* pool_v, int kv_dtype,
@@ -867,9 +826,12 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
   if ((uintptr_t)pool_k % 16 || (uintptr_t)pool_v % 16 || (uintptr_t)q % 16 || (uintptr_t)out % 16)
     return set_error(KVE_ERR_ARG, "%s: q, out and the pools must be 16-byte aligned", me);
   const Split s = split_of(batch, max_q_len, max_ctx, num_kv_heads, group);
-  const size_t part = partial_bytes(s, batch, num_kv_heads, head_dim);
-  if (part && (!workspace || workspace_bytes < kCounterBytes + part))
-    return set_error(KVE_ERR_WORKSPACE, "%s: workspace needs %zu bytes", me, kCounterBytes + part);
+  const bool wide = kv_dtype == KVE_BF16 && use_wide(max_q_len, group) && block_size % 16 == 0 &&
+                    num_blocks * block_size < (1ll << 31) - 16;
+  const size_t part = wide ? tree_attn_wide_partial_bytes(batch, max_q_len, max_ctx, num_kv_heads, group, head_dim)
+                           : partial_bytes(s, batch, num_kv_heads, head_dim);
+  if (part && (!workspace || workspace_bytes < kTreeCounterBytes + part))
+    return set_error(KVE_ERR_WORKSPACE, "%s: workspace needs %zu bytes", me, kTreeCounterBytes + part);
   if (part && (uintptr_t)workspace % 16) return set_error(KVE_ERR_ARG, "%s: workspace must be 16-byte aligned", me);
   TreeParams p{};
   p.q = q; p.pool_k = pool_k; p.pool_v = pool_v; p.k_scale = k_scale; p.v_scale = v_scale;
@@ -879,8 +841,9 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
   p.max_q = max_q_len; p.nq = num_heads; p.nkv = num_kv_heads; p.group = group; p.bs = block_size;
   p.num_blocks = num_blocks; p.scale = scale; p.out = out;
   p.counters = static_cast<int*>(workspace);
-  p.partials = part ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes) : nullptr;
+  p.partials = part ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kTreeCounterBytes) : nullptr;
   p.chunk = s.chunk; p.n_chunks = s.n_chunks; p.n_qtiles = s.n_qtiles; p.status = dev_status;
+  if (wide) return tree_attn_wide(p, batch, max_ctx, head_dim, stream);
   if (kv_dtype == KVE_FP8_E4M3) return launch_hd<kFp8>(p, head_dim, s.rb, batch, stream);
   if (dtype == KVE_BF16) return launch_hd<kBf16>(p, head_dim, s.rb, batch, stream);
   return launch_hd<kF32>(p, head_dim, s.rb, batch, stream);

@@ -1,0 +1,704 @@
+// Tree attention for many query rows per kv head, on the 5th-generation tensor cores.
+//
+// The same operation as tree_attn.cu for bf16 caches, where a sequence's tree has more
+// rows (nodes x group heads) than the tile of m16 products can hide: the work is then
+// bound by the tensor cores and the exponentials rather than by the cache's bytes.
+//
+// A CTA has two softmax warpgroups, each with its own 128-row score tile S and output
+// tile O in tensor memory, and one of two jobs:
+//   one query tile (up to 128 rows): the two groups take the even and the odd key tiles
+//     of the chunk, and their outputs are joined at the end;
+//   two query tiles (up to 256 rows): both groups take every key tile, one query tile
+//     each, so that a K/V tile is fetched into shared memory once for 256 rows.
+// Either way the tensor cores work on one group's tile while the other group is in its
+// softmax. Per key tile (128 keys) and group:
+//   S = Q K^T      tcgen05.mma, Q and K in shared memory (128-byte swizzle, K-major)
+//   P = 2^(S sl - m)  one thread a row: a pass for the maximum, a pass for the exponentials;
+//                  P goes back to tensor memory as bf16, over S
+//   O += P V       tcgen05.mma, P from tensor memory, V from shared memory as it lies there
+//                  (keys x dims: the transposed, MN-major form)
+// O is rescaled only where the running maximum has grown by more than 2^8 since its
+// last use: until then P is at most 2^8, which bf16 and fp32 hold as well as 1.
+//
+// K and V tiles come by TMA in boxes of 16 keys x 64 dims (so blocks of any multiple of
+// 16 positions), through a ring of slots in the order in which the products use them.
+// One more warp looks at every V tile before it is used: rows behind the last key are
+// zeroed (the pool's contents there are not this sequence's), and new tokens' rows are
+// checked for infinities and NaN, which 0 x V would spread to rows that do not see them.
+// Where there are any, the chunk's rows are computed again, key by key.
+#include <math.h>
+
+#include <atomic>
+#include <cstring>
+
+#include "kve_common.cuh"
+#include "tma.cuh"
+#include "tree_attn.cuh"
+
+namespace kve {
+namespace {
+
+constexpr int kKeys = 128;       // keys of a tile
+constexpr int kRows = 128;       // query rows of a tile
+constexpr int kThreads = 384;    // loader, MMA issuer, V warp, TMEM warp; two softmax warpgroups
+constexpr int kMaxSlots = 8;
+
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+// V as it lies: 64-dim halves `half_bytes` apart, 8-key groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t half_bytes) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)((half_bytes >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16, fp32 accumulator, bf16 operands, M = 128; b_mn: B is MN-major.
+__device__ __forceinline__ uint32_t mma_idesc(int n, bool b_mn) {
+  return 1u << 4 | 1u << 7 | 1u << 10 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kRows >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const float (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+      "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
+      "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+      "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15])),
+      "r"(__float_as_uint(v[16])), "r"(__float_as_uint(v[17])), "r"(__float_as_uint(v[18])), "r"(__float_as_uint(v[19])),
+      "r"(__float_as_uint(v[20])), "r"(__float_as_uint(v[21])), "r"(__float_as_uint(v[22])), "r"(__float_as_uint(v[23])),
+      "r"(__float_as_uint(v[24])), "r"(__float_as_uint(v[25])), "r"(__float_as_uint(v[26])), "r"(__float_as_uint(v[27])),
+      "r"(__float_as_uint(v[28])), "r"(__float_as_uint(v[29])), "r"(__float_as_uint(v[30])), "r"(__float_as_uint(v[31]))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ bool odd_bits(uint32_t w) {
+  return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+}
+
+// TWO: two query tiles, both groups on every key tile; else one, groups on alternate tiles.
+template <int HD, bool TWO>
+struct WideShape {
+  static constexpr int QT = TWO ? 2 : 1;
+  static constexpr int QBYTES = kRows * HD * 2;
+  static constexpr int SLOT = kKeys * HD * 2;
+  static constexpr int NS = HD == 128 ? (TWO ? 5 : 6) : 8;
+  static constexpr int XROW = HD + 4;  // floats of a row of the joining area (in the ring)
+  static constexpr int BARS = (3 * kMaxSlots + 6) * 8;
+  static constexpr size_t SMEM = 1024 + (size_t)QT * QBYTES + (size_t)NS * SLOT + BARS + 64;
+  static_assert(NS * SLOT >= kRows * (XROW + 2) * 4, "joining area");
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+template <int HD, bool TWO>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeParams p) {
+  using W = WideShape<HD, TWO>;
+  constexpr int NS = W::NS, HALVES = HD / 64;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_smem = smem;
+  uint8_t* ring = smem + W::QT * W::QBYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + (size_t)NS * W::SLOT);
+  uint64_t* full = bars;                     // a slot's TMA bytes have landed
+  uint64_t* ready = bars + kMaxSlots;        // by V tile (mod NS): the V warp has been over it
+  uint64_t* empty = bars + 2 * kMaxSlots;    // the products that read it are done
+  uint64_t* s_ready = bars + 3 * kMaxSlots;  // by group: S is complete
+  uint64_t* p_ready = s_ready + 2;           // P is in tensor memory (one arrival a warp)
+  uint64_t* o_ready = s_ready + 4;           // O is complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kMaxSlots + 6);
+  int* odd = reinterpret_cast<int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(smem_u32(&full[i]), 1);
+      mbar_init(smem_u32(&ready[i]), 1);
+      mbar_init(smem_u32(&empty[i]), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(smem_u32(&s_ready[g]), 1);
+      mbar_init(smem_u32(&p_ready[g]), 4);
+      mbar_init(smem_u32(&o_ready[g]), 1);
+    }
+    *odd = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+  }
+  grid_dep_wait();
+  grid_dep_launch();
+
+  const int bh = blockIdx.x, c = blockIdx.y, qtile = blockIdx.z;
+  const int b = bh / p.nkv, h = bh % p.nkv;
+  const int ctx = p.ctx_lens[b], ql = p.q_lens[b], qoff = p.q_offsets[b];
+  if (ql < 0 || ql > p.max_q || ctx < ql || qoff < 0 || (int64_t)ctx > (int64_t)p.table_stride * p.bs ||
+      (int64_t)ctx > (int64_t)p.chunk * p.n_chunks) {
+    if (threadIdx.x == 0 && c == 0 && qtile == 0) report(p.status, KVE_ERR_BOUNDS);
+    return;
+  }
+  const int row0 = qtile * W::QT * kRows;
+  const int rows = min(W::QT * kRows, ql * p.group - row0);
+  if (rows <= 0) return;
+  const int hist = ctx - ql;
+  const int key_end = p.mask ? ctx : hist + (row0 + rows - 1) / p.group + 1;
+  const int live = (key_end + p.chunk - 1) / p.chunk;
+  if (c >= live) return;
+  const int key_lo = c * p.chunk;
+  const int key_hi = min(key_end, key_lo + p.chunk);
+  const int n = (key_hi - key_lo + kKeys - 1) / kKeys;  // key tiles
+  // Steps of group g, and the key tile of its step i.
+  const int steps0 = TWO ? n : (n + 1) / 2, steps1 = TWO ? (rows > kRows ? n : 0) : n / 2;
+  auto steps = [&](int g) { return g ? steps1 : steps0; };
+  auto tile_of = [&](int g, int i) { return TWO ? i : 2 * i + g; };
+  // The ring's order is the order of use. TWO: K0 V0 K1 V1 ..; else K0 K1 V0 K2 V1 .. V(n-2) V(n-1).
+  auto k_item = [&](int t) { return TWO ? 2 * t : t < 2 ? t : 2 * t - 1; };
+  auto v_item = [&](int t) { return TWO ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1); };
+
+  if (warp == 3) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q);
+  auto head_row = [&](int r) {  // row r of the CTA in q and out
+    const int gr = row0 + r;
+    return ((size_t)(qoff + gr / p.group) * p.nq + h * p.group + gr % p.group) * HD;
+  };
+  if (warp >= 4) {
+    // Q into shared memory, 16 bytes a lane; a negative scale is a sign on q.
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+    for (int i = threadIdx.x - 128; i < W::QT * kRows * (HD / 8); i += 256) {
+      const int r = i / (HD / 8), ch = i % (HD / 8);
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows) x = *reinterpret_cast<const uint4*>(q + head_row(r) + ch * 8);
+      x.x ^= flip;
+      x.y ^= flip;
+      x.z ^= flip;
+      x.w ^= flip;
+      const int rr = r % kRows;
+      uint8_t* dst = q_smem + (r / kRows) * W::QBYTES + (ch / 8) * (kRows * 128) + rr * 128 + (((ch % 8) ^ (rr & 7)) << 4);
+      *reinterpret_cast<uint4*>(dst) = x;
+    }
+    fence_proxy_async_smem();
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = *tmem_slot;
+  auto s_col = [&](int g) { return tmem + (uint32_t)(g * 128); };
+  auto o_col = [&](int g) { return tmem + (uint32_t)(256 + g * 128); };
+  auto slot_addr = [&](int item) { return smem_u32(ring) + (uint32_t)((item % NS) * W::SLOT); };
+  bool ok = true;  // no wait of this thread has run out
+  const int items = 2 * n;
+
+  float m = -INFINITY, l = 0.f;  // softmax threads: the row's base and its sum
+  const int grp = warp >= 8 ? 1 : 0, row = (warp & 3) * 32 + lane;
+  if (warp == 0) {
+    // ---- loader: lanes 0 .. 7 ask for 16 keys each
+    const int32_t* table = p.tables + (size_t)b * p.table_stride;
+    const int past = (int)(p.num_blocks * p.bs);  // rows from here on load as zeros
+    auto load = [&](const CUtensorMap* map, int t, int item) {
+      const int slot = item % NS;
+      if (item >= NS) ok = ok && mbar_wait(smem_u32(&empty[slot]), (uint32_t)(item / NS - 1) & 1u, p.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      if (lane == 0) mbar_expect_tx(smem_u32(&full[slot]), W::SLOT);
+      __syncwarp();
+      if (lane < 8) {
+        const int key = key_lo + t * kKeys + lane * 16;
+        int y = past;
+        if (key < key_hi) {
+          const int blk = table[key / p.bs];
+          if (blk >= 0 && blk < p.num_blocks) y = (int)((int64_t)blk * p.bs + key % p.bs);
+          else report(p.status, KVE_ERR_BOUNDS);
+        }
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half)
+          tma_load_2d(slot_addr(item) + half * (kKeys * 128) + lane * 2048, map, h * HD + half * 64, y, smem_u32(&full[slot]));
+      }
+      __syncwarp();
+    };
+    int done = 0;
+    for (int item = 0; item < items && ok; ++item) {
+      // which tile's K or V comes next
+      int t;
+      bool is_k;
+      if (TWO) {
+        t = item / 2;
+        is_k = item % 2 == 0;
+      } else if (item < 2) {
+        t = n == 1 ? 0 : item;
+        is_k = n > 1 || item == 0;
+      } else {
+        is_k = item % 2 == 1 && item != items - 1;
+        t = is_k ? (item + 1) / 2 : item == items - 1 ? n - 1 : item / 2 - 1;
+      }
+      load(is_k ? &map_k : &map_v, t, item);
+      done = item + 1;
+    }
+    if (!ok)  // let what is in flight land
+      for (int item = max(0, done - NS); item < done; ++item)
+        mbar_wait(smem_u32(&full[item % NS]), (uint32_t)(item / NS) & 1u, p.status);
+  } else if (warp == 1) {
+    // ---- MMA issuer
+    if (lane == 0) {
+      const uint32_t id_qk = mma_idesc(kKeys, false), id_pv = mma_idesc(HD, true);
+      const int last_user = TWO ? (steps1 ? 1 : 0) : -1;  // TWO: the group whose product is a slot's last
+      auto qk = [&](int g, int i) {
+        const int item = k_item(tile_of(g, i)), slot = item % NS;
+        ok = ok && mbar_wait(smem_u32(&full[slot]), (uint32_t)(item / NS) & 1u, p.status);
+        if (!ok) return;
+        tc_after();
+        const uint64_t ad = desc_k_major(smem_u32(q_smem) + (TWO ? g * W::QBYTES : 0)), bd = desc_k_major(slot_addr(item));
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint64_t step = (uint64_t)((kk / 4) * (kKeys * 128 / 16) + (kk % 4) * 2);
+          mma_ss(s_col(g), ad + step, bd + step, id_qk, kk > 0);
+        }
+        if (!TWO || g == last_user) mma_commit(smem_u32(&empty[slot]));
+        mma_commit(smem_u32(&s_ready[g]));
+      };
+      auto pv = [&](int g, int i) {
+        const int t = tile_of(g, i), item = v_item(t), slot = item % NS;
+        ok = ok && mbar_wait(smem_u32(&p_ready[g]), (uint32_t)i & 1u, p.status);
+        ok = ok && mbar_wait(smem_u32(&full[slot]), (uint32_t)(item / NS) & 1u, p.status);
+        ok = ok && mbar_wait(smem_u32(&ready[t % NS]), (uint32_t)(t / NS) & 1u, p.status);
+        if (!ok) return;
+        tc_after();
+        const uint64_t bd = desc_mn_major(slot_addr(item), kKeys * 128);
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_ts(o_col(g), s_col(g) + kk * 8, bd + (uint64_t)(kk * (2048 / 16)), id_pv, i > 0 || kk > 0);
+        if (!TWO || g == last_user) mma_commit(smem_u32(&empty[slot]));
+      };
+      for (int g = 0; g < 2; ++g)
+        if (steps(g) > 0) qk(g, 0);
+      for (int i = 0; i < steps0 && ok; ++i)
+        for (int g = 0; g < 2; ++g) {
+          if (i >= steps(g)) continue;
+          pv(g, i);
+          if (i + 1 < steps(g)) qk(g, i + 1);
+          else mma_commit(smem_u32(&o_ready[g]));
+        }
+      if (!ok) {  // end what was issued before the memory it uses goes away
+        mma_commit(smem_u32(&o_ready[0]));
+        mbar_wait(smem_u32(&o_ready[0]), 0, p.status);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ---- V: zero rows behind the last key, look for infinities and NaN in new tokens' rows
+    for (int t = 0; t < n && ok; ++t) {
+      const int item = v_item(t), slot = item % NS;
+      ok = ok && mbar_wait(smem_u32(&full[slot]), (uint32_t)(item / NS) & 1u, p.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const int kt = key_lo + t * kKeys;
+      uint8_t* v = ring + (size_t)slot * W::SLOT;
+      if (kt + kKeys > key_hi) {
+        const int first = key_hi - kt, stop = min(kKeys, (first + 15) / 16 * 16);  // further boxes are zeros already
+        for (int i = lane; i < (stop - first) * 8 * HALVES; i += 32) {
+          const int half = i / ((stop - first) * 8), rem = i % ((stop - first) * 8);
+          *reinterpret_cast<uint4*>(v + half * (kKeys * 128) + (first + rem / 8) * 128 + rem % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+      const int r0 = max(hist - kt, 0), r1 = min(kKeys, key_hi - kt);
+      if (r0 < r1) {
+        bool found = false;
+        for (int i = lane; i < (r1 - r0) * 8 * HALVES; i += 32) {
+          const int half = i / ((r1 - r0) * 8), rem = i % ((r1 - r0) * 8);
+          const uint4 x = *reinterpret_cast<const uint4*>(v + half * (kKeys * 128) + (r0 + rem / 8) * 128 + rem % 8 * 16);
+          found |= odd_bits(x.x) || odd_bits(x.y) || odd_bits(x.z) || odd_bits(x.w);
+        }
+        if (__any_sync(0xffffffffu, found) && lane == 0) *odd = 1;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ready[t % NS]));
+    }
+  } else if (warp >= 4) {
+    // ---- softmax: a thread a row
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int r = (TWO ? grp * kRows : 0) + row;  // row of the CTA
+    const bool active = (TWO ? grp * kRows : 0) + (warp & 3) * 32 < rows;  // any row of this warp
+    const int node = (row0 + min(r, rows - 1)) / p.group;
+    const uint32_t* mask = p.mask ? p.mask + (size_t)(qoff + node) * p.mask_words : nullptr;
+    const float sl = fabsf(p.scale) * 1.4426950408889634f;
+    const int my_steps = steps(grp);
+    for (int i = 0; i < my_steps; ++i) {
+      ok = ok && mbar_wait(smem_u32(&s_ready[grp]), (uint32_t)i & 1u, p.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (active) {
+        tc_after();
+        const int kt = key_lo + tile_of(grp, i) * kKeys;
+        const bool masked = kt + kKeys > hist || kt + kKeys > key_hi;
+        uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+        if (masked) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int at = kt + 32 * w;
+            see[w] = p.mask ? mask_bits<32>(mask, p.mask_words, at - hist) : chain_bits(node, at - hist);
+            const int in = key_hi - at;
+            see[w] &= in >= 32 ? ~0u : in <= 0 ? 0u : (1u << in) - 1u;
+          }
+        }
+        const uint32_t sc = s_col(grp) + lanes;
+        float top = -INFINITY;
+        float v[32];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          tmem_load(sc + 32 * w, v);
+          if (masked) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) top = fmaxf(top, see[w] >> x & 1 ? v[x] : -INFINITY);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) top = fmaxf(top, v[x]);
+          }
+        }
+        top *= sl;  // 0 x infinity: NaN, and no new base
+        const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? ex2(m - top) : 1.f;
+          if (grow) m = top;
+          l *= f;
+          if (i > 0) {
+#pragma unroll 1
+            for (int w = 0; w < HD / 32; ++w) {
+              tmem_load(o_col(grp) + lanes + 32 * w, v);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) v[x] *= f;
+              tmem_store32(o_col(grp) + lanes + 32 * w, v);
+            }
+          }
+        }
+        const float off = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          tmem_load(sc + 32 * w, v);
+          uint32_t packed[16];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            float e = fmaf(v[x], sl, off);
+            if (masked) e = see[w] >> x & 1 ? e : -INFINITY;
+            v[x] = ex2(e);
+            sum[x & 3] += v[x];
+          }
+#pragma unroll
+          for (int x = 0; x < 16; ++x) packed[x] = pack2(v[2 * x], v[2 * x + 1]);
+          tmem_store16(sc + 16 * w, packed);  // over columns of S already read
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_store_wait();
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&p_ready[grp]));
+    }
+    if (my_steps > 0) ok = ok && mbar_wait(smem_u32(&o_ready[grp]), 0, p.status);
+    tc_after();
+  }
+  // Every role is done; a wait that ran out anywhere leaves the outputs unwritten.
+  const bool failed = __syncthreads_or(!ok);
+
+  constexpr int PROW = HD + 4;
+  constexpr int TILE_ROWS = W::QT * kRows;
+  float* part0 = p.partials + ((size_t)bh * p.n_qtiles + qtile) * p.n_chunks * TILE_ROWS * PROW;
+  float* part = part0 + (size_t)c * TILE_ROWS * PROW;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
+  float* xs = reinterpret_cast<float*>(ring);  // the second group's rows: O, then m and l
+  const bool recompute = *odd != 0;
+  if (!failed && !recompute && warp >= 4) {
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    float* xr = xs + (size_t)row * W::XROW;
+    float* xml = xs + (size_t)kRows * W::XROW + row * 2;
+    float v[32];
+    if (!TWO && grp == 1) {
+      // hand over to the first group
+      if (steps1 > 0 && (warp & 3) * 32 < rows) {
+#pragma unroll 1
+        for (int w = 0; w < HD / 32; ++w) {
+          tmem_load(o_col(1) + lanes + 32 * w, v);
+#pragma unroll
+          for (int x = 0; x < 32; x += 4)
+            *reinterpret_cast<float4*>(xr + 32 * w + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+        }
+      }
+      *reinterpret_cast<float2*>(xml) = make_float2(m, l);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    } else {
+      float f0 = 1.f, f1 = 0.f;
+      if (!TWO) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float2 ml = *reinterpret_cast<const float2*>(xml);
+        const float t = fmaxf(m, ml.x);
+        f0 = m == t ? 1.f : ex2(m - t);
+        f1 = ml.x == t ? 1.f : ex2(ml.x - t);
+        m = t;
+        l = l * f0 + ml.y * f1;
+      }
+      const int r = (TWO ? grp * kRows : 0) + row;
+      if ((TWO ? grp * kRows : 0) + (warp & 3) * 32 < rows) {
+        const bool join = !TWO && steps1 > 0;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int w = 0; w < HD / 32; ++w) {
+          tmem_load(o_col(TWO ? grp : 0) + lanes + 32 * w, v);
+          if (join) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 4) {
+              const float4 y = *reinterpret_cast<const float4*>(xr + 32 * w + x);
+              v[x] = v[x] * f0 + y.x * f1;
+              v[x + 1] = v[x + 1] * f0 + y.y * f1;
+              v[x + 2] = v[x + 2] * f0 + y.z * f1;
+              v[x + 3] = v[x + 3] * f0 + y.w * f1;
+            }
+          }
+          if (r < rows && live == 1) {
+            __nv_bfloat16* dst = out + head_row(r) + 32 * w;
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+              uint4 o;
+              o.x = pack2(l == 0.f ? 0.f : v[x] * inv, l == 0.f ? 0.f : v[x + 1] * inv);
+              o.y = pack2(l == 0.f ? 0.f : v[x + 2] * inv, l == 0.f ? 0.f : v[x + 3] * inv);
+              o.z = pack2(l == 0.f ? 0.f : v[x + 4] * inv, l == 0.f ? 0.f : v[x + 5] * inv);
+              o.w = pack2(l == 0.f ? 0.f : v[x + 6] * inv, l == 0.f ? 0.f : v[x + 7] * inv);
+              *reinterpret_cast<uint4*>(dst + x) = o;
+            }
+          } else if (r < rows) {
+            float* dst = part + (size_t)r * PROW + 32 * w;
+#pragma unroll
+            for (int x = 0; x < 32; x += 4)
+              *reinterpret_cast<float4*>(dst + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+          }
+          __syncwarp();  // the loads of tensor memory are the whole warp's
+        }
+        if (live > 1 && r < rows) *reinterpret_cast<float2*>(part + (size_t)r * PROW + HD) = make_float2(m, l);
+      }
+    }
+  }
+  if (!failed && recompute) {
+    // Key by key over what each row sees: a warp a row, HD / 32 dims a lane.
+    constexpr int DPL = HD / 32;
+    const int32_t* table = p.tables + (size_t)b * p.table_stride;
+    const __nv_bfloat16* pk = static_cast<const __nv_bfloat16*>(p.pool_k);
+    const __nv_bfloat16* pv = static_cast<const __nv_bfloat16*>(p.pool_v);
+    const float sl = p.scale * 1.4426950408889634f;
+    for (int r = warp; r < rows; r += kThreads / 32) {
+      const int node = (row0 + r) / p.group;
+      const uint32_t* mask = p.mask ? p.mask + (size_t)(qoff + node) * p.mask_words : nullptr;
+      float qv[DPL], acc[DPL] = {};
+#pragma unroll
+      for (int d = 0; d < DPL; ++d) qv[d] = __bfloat162float(q[head_row(r) + lane + 32 * d]);
+      float rm = -INFINITY, rl = 0.f;
+      for (int key = key_lo; key < key_hi; ++key) {
+        const int j = key - hist;
+        if (j >= 0 && !(mask ? mask_bits<1>(mask, p.mask_words, j) & 1u : j <= node)) continue;
+        const int blk = table[key / p.bs];
+        const bool in = blk >= 0 && blk < p.num_blocks;  // reported by the loader
+        const size_t at = in ? (((size_t)blk * p.bs + key % p.bs) * p.nkv + h) * HD : 0;
+        float s = 0.f;
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) s += in ? qv[d] * __bfloat162float(pk[at + lane + 32 * d]) : 0.f;
+        s = warp_sum(s) * sl;
+        if (s > rm) {
+          const float f = ex2(rm - s);
+          rm = s;
+          rl *= f;
+#pragma unroll
+          for (int d = 0; d < DPL; ++d) acc[d] *= f;
+        }
+        const float e = s == -INFINITY ? 0.f : ex2(s - rm);
+        rl += e;
+#pragma unroll
+        for (int d = 0; d < DPL; ++d)
+          if (e != 0.f) acc[d] += in ? e * __bfloat162float(pv[at + lane + 32 * d]) : 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < DPL; ++d) {
+        if (live == 1) out[head_row(r) + lane + 32 * d] = __float2bfloat16_rn(rl == 0.f ? 0.f : acc[d] / rl);
+        else part[(size_t)r * PROW + lane + 32 * d] = acc[d];
+      }
+      if (live > 1 && lane == 0) *reinterpret_cast<float2*>(part + (size_t)r * PROW + HD) = make_float2(rm, rl);
+    }
+  }
+  tc_before();
+  __threadfence();
+  __syncthreads();
+  if (warp == 3) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+  if (live == 1) return;
+
+  // The last of the tile's chunks to arrive joins them, in chunk order.
+  int* last = odd;  // its value has been read by all
+  if (threadIdx.x == 0) {
+    int* cnt = p.counters + (size_t)bh * p.n_qtiles + qtile;
+    *last = atomicAdd(cnt, 1) == live - 1;
+    if (*last) *cnt = 0;  // the workspace is left as it was
+  }
+  __syncthreads();
+  if (!*last || failed) return;
+  __threadfence();
+  for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
+    const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+    const float* pr = part0 + (size_t)r * PROW;
+    float rm = -INFINITY, rl = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < live; ++s) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(pr + (size_t)s * TILE_ROWS * PROW + HD));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(pr + (size_t)s * TILE_ROWS * PROW + d));
+      const float t = fmaxf(rm, ml.x);
+      const float f = t == rm ? 1.f : ex2(rm - t), w = t == ml.x ? 1.f : ex2(ml.x - t);
+      rm = t;
+      rl = rl * f + ml.y * w;
+      o.x = o.x * f + x.x * w;
+      o.y = o.y * f + x.y * w;
+      o.z = o.z * f + x.z * w;
+      o.w = o.w * f + x.w * w;
+    }
+    const bool none = rl == 0.f;
+    *reinterpret_cast<uint2*>(out + head_row(r) + d) =
+        make_uint2(pack2(none ? 0.f : o.x / rl, none ? 0.f : o.y / rl), pack2(none ? 0.f : o.z / rl, none ? 0.f : o.w / rl));
+  }
+}
+
+// ------------------------------------------------------------------ host
+struct WidePlan {
+  bool two;
+  int n_qtiles, chunk, n_chunks;
+};
+
+// One or two query tiles a CTA by the rows of the call's largest tree, and the number
+// of chunks that costs least: waves of one CTA an SM, each a fixed part (launch, Q,
+// the first tile's latency, joining: about 5 us) and a part per step (about 1.4 us).
+WidePlan wide_plan(int batch, int max_q, int max_ctx, int nkv, int group) {
+  WidePlan w;
+  const long long rows = (long long)max_q * group;
+  w.two = rows > kRows;
+  const int per = (w.two ? 2 : 1) * kRows;
+  w.n_qtiles = (int)((rows + per - 1) / per);
+  const long long units = (long long)batch * nkv * w.n_qtiles;
+  const int tiles = (max_ctx + kKeys - 1) / kKeys;
+  double best = 1e30;
+  w.chunk = tiles * kKeys;
+  w.n_chunks = 1;
+  for (int c = 1; c <= tiles && c <= 32; ++c) {
+    const int per_chunk = (tiles + c - 1) / c, chunks = (tiles + per_chunk - 1) / per_chunk;
+    if (chunks != c || (c > 1 && units > (long long)kTreeCounterSlots)) continue;
+    const int steps = w.two ? per_chunk : (per_chunk + 1) / 2;
+    const double waves = (double)((units * c + 147) / 148);
+    const double t = waves * (5.0 + 1.4 * steps) + (c > 1 ? 2.0 + 0.15 * c : 0.0);
+    if (t < best) {
+      best = t;
+      w.chunk = per_chunk * kKeys;
+      w.n_chunks = c;
+    }
+  }
+  return w;
+}
+
+bool pool_map(CUtensorMap* map, const void* pool, int64_t rows, int width) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || width >= (1 << 24)) return false;
+  return cached_map(map, pool, (uint64_t)rows | (uint64_t)width << 32, [&](CUtensorMap* m) {
+    cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)width * 2};
+    cuuint32_t box[2] = {64, 16};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  });
+}
+
+template <int HD, bool TWO>
+int launch(const TreeParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int batch, cudaStream_t stream) {
+  using W = WideShape<HD, TWO>;
+  static std::atomic<uint64_t> prepared{0};  // the shared-memory limit is an attribute of the kernel on one device
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (err == cudaSuccess && !(prepared.load(std::memory_order_relaxed) & bit)) {
+    err = cudaFuncSetAttribute(tree_attn_wide_kernel<HD, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W::SMEM);
+    if (err == cudaSuccess) prepared.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(KVE_ERR_CUDA, "kve_paged_tree_attn: %s", cudaGetErrorString(err));
+  }
+  launch_kernel(tree_attn_wide_kernel<HD, TWO>, dim3(batch * p.nkv, p.n_chunks, p.n_qtiles), dim3(kThreads), W::SMEM, stream,
+                mk, mv, p);
+  return check_launch("kve_paged_tree_attn(wide)");
+}
+
+}  // namespace
+
+size_t tree_attn_wide_partial_bytes(int batch, int max_q, int max_ctx, int nkv, int group, int hd) {
+  const WidePlan w = wide_plan(batch, max_q, max_ctx, nkv, group);
+  if (w.n_chunks == 1) return 0;
+  return (size_t)batch * nkv * w.n_qtiles * w.n_chunks * ((w.two ? 2 : 1) * kRows) * (hd + 4) * sizeof(float);
+}
+
+int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, cudaStream_t stream) {
+  const WidePlan w = wide_plan(batch, p.max_q, max_ctx, p.nkv, p.group);
+  p.chunk = w.chunk;
+  p.n_chunks = w.n_chunks;
+  p.n_qtiles = w.n_qtiles;
+  CUtensorMap mk, mv;
+  memset(&mk, 0, sizeof(mk));
+  memset(&mv, 0, sizeof(mv));
+  const int64_t rows = p.num_blocks * p.bs;
+  if (!pool_map(&mk, p.pool_k, rows, p.nkv * hd) || !pool_map(&mv, p.pool_v, rows, p.nkv * hd))
+    return set_error(KVE_ERR_CUDA, "kve_paged_tree_attn: no tensor map for the pool");
+  if (hd == 64) return w.two ? launch<64, true>(p, mk, mv, batch, stream) : launch<64, false>(p, mk, mv, batch, stream);
+  return w.two ? launch<128, true>(p, mk, mv, batch, stream) : launch<128, false>(p, mk, mv, batch, stream);
+}
+
+}  // namespace kve

@@ -153,6 +153,26 @@ def test_tree_attention_long_histories_are_split_and_joined(cuda_device, cache, 
     assert torch.equal(ops.tree_attention(**args, workspace=ws), got)
 
 
+@pytest.mark.parametrize("heads", [(14, 2, 64), (16, 2, 128), (3, 3, 64), (64, 1, 128)])
+@pytest.mark.parametrize("nodes, hists, bs, kind", [
+    ([45], [0], 16, "tree"),                     # the tree alone
+    ([50, 64, 7], [300, 129, 128], 16, "tree"),  # histories around a key tile's end
+    ([130, 1, 40], [33, 700, 0], 32, "random"),  # rows without keys, masks of five words
+    ([64, 64], [63, 1000], 48, "none"),          # chains
+    ([33, 0, 35], [2500, 5, 90], 16, "tree"),    # split into chunks, a sequence without new tokens
+])
+def test_tree_attention_many_rows(cuda_device, heads, nodes, hists, bs, kind):
+    """Trees of more rows than one tensor-core tile, in every arrangement of tiles and chunks."""
+    args, *lens = attention_case("bf16", heads, nodes, hists, bs, kind, 17, cuda_device)
+    status = ops.status_tensor(cuda_device)
+    ws = ops.Workspace(cuda_device)
+    got = ops.tree_attention(**args, workspace=ws, status=status)
+    check_attention(args, *lens, got)
+    assert int(status) == 0 and int(ws.buf[:65536].view(torch.int32).abs().sum()) == 0
+    assert torch.equal(ops.tree_attention(**args, workspace=ws), got)
+    check_attention(dict(args, scale=-0.05), *lens, ops.tree_attention(**dict(args, scale=-0.05)))
+
+
 def test_tree_attention_joins_with_extreme_scores(cuda_device):
     """Scores hundreds apart between chunks and streams: shares of exactly 0 and 1, no overflow."""
     for cache in ("bf16", "fp32", "fp8"):
