@@ -219,10 +219,10 @@ tree_attn_kernel(TreeParams p) {
   // Query rows of this warp: g and g + 8 of its row block.
   const QT* q = static_cast<const QT*>(p.q);
   const int r_lo = rb * 16 + g, r_hi = r_lo + 8;
-  const int n_lo = (row0 + r_lo) / p.group, n_hi = (row0 + r_hi) / p.group;  // nodes
+  const int n_lo = node_of(p, row0 + r_lo), n_hi = node_of(p, row0 + r_hi);
   auto q_row = [&](int r) {
-    const int gr = row0 + r;
-    return q + ((size_t)(qoff + gr / p.group) * p.nq + h * p.group + gr % p.group) * HD;
+    const int gr = row0 + r, node = node_of(p, gr);
+    return q + ((size_t)(qoff + node) * p.nq + h * p.group + gr - node * p.group) * HD;
   };
   constexpr int KSTEPS = HD / 16;
   uint32_t qa[KV == kF32 ? 1 : KSTEPS][4];
@@ -641,8 +641,8 @@ tree_attn_kernel(TreeParams p) {
     o.y = l == 0.f ? 0.f : o.y / l;
     o.z = l == 0.f ? 0.f : o.z / l;
     o.w = l == 0.f ? 0.f : o.w / l;
-    const int gr = row0 + r;
-    QT* dst = out + ((size_t)(qoff + gr / p.group) * p.nq + h * p.group + gr % p.group) * HD + d;
+    const int gr = row0 + r, node = node_of(p, gr);
+    QT* dst = out + ((size_t)(qoff + node) * p.nq + h * p.group + gr - node * p.group) * HD + d;
     if constexpr (KV == kF32) *reinterpret_cast<float4*>(dst) = o;
     else *reinterpret_cast<uint2*>(dst) = make_uint2(bf16x2(o.x, o.y), bf16x2(o.z, o.w));
   };
@@ -813,6 +813,7 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
     return set_error(KVE_ERR_SHAPE, "%s: head_dim %d (supported: 64, 128)", me, head_dim);
   const int group = num_heads / num_kv_heads;
   if (group > kMaxGroup) return set_error(KVE_ERR_SHAPE, "%s: group %d > %d", me, group, kMaxGroup);
+  if (num_blocks > 0x7fffffffLL / block_size) return set_error(KVE_ERR_SHAPE, "%s: more than 2^31 slots", me);
   if (max_q_len > kMaxNodes) return set_error(KVE_ERR_SHAPE, "%s: max_q_len %d > %d", me, max_q_len, kMaxNodes);
   if ((long long)batch * num_kv_heads > 0x7fffffffLL) return set_error(KVE_ERR_SHAPE, "%s: batch too large", me);
   if (dtype != KVE_F32 && dtype != KVE_BF16) return set_error(KVE_ERR_DTYPE, "%s: dtype %d", me, dtype);
@@ -827,7 +828,7 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
     return set_error(KVE_ERR_ARG, "%s: q, out and the pools must be 16-byte aligned", me);
   const Split s = split_of(batch, max_q_len, max_ctx, num_kv_heads, group);
   const bool wide = kv_dtype == KVE_BF16 && use_wide(max_q_len, group) && block_size % 16 == 0 &&
-                    num_blocks * block_size < (1ll << 31) - 16;
+                    num_blocks * block_size < 0x7ffffff0LL;
   const size_t part = wide ? tree_attn_wide_partial_bytes(batch, max_q_len, max_ctx, num_kv_heads, group, head_dim)
                            : partial_bytes(s, batch, num_kv_heads, head_dim);
   if (part && (!workspace || workspace_bytes < kTreeCounterBytes + part))
@@ -839,6 +840,7 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
   p.ctx_lens = ctx_lens; p.q_lens = q_lens; p.q_offsets = q_offsets;
   p.mask = tree_mask; p.mask_words = mask_words;
   p.max_q = max_q_len; p.nq = num_heads; p.nkv = num_kv_heads; p.group = group; p.bs = block_size;
+  p.group_inv = (uint32_t)((1ull << 32) / (uint32_t)group + 1);
   p.num_blocks = num_blocks; p.scale = scale; p.out = out;
   p.counters = static_cast<int*>(workspace);
   p.partials = part ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kTreeCounterBytes) : nullptr;

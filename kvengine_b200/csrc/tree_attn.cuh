@@ -31,11 +31,17 @@ struct TreeParams {
   int* counters;
   float* partials;
   int chunk, n_chunks, n_qtiles;
+  uint32_t group_inv;  // floor(2^32 / group) + 1: r / group = umulhi(r, it) for r < 2^16 (group 1: not used)
   int* status;
 };
 
+// Row r (below 2^16) of a sequence and kv head: its node.
+__device__ __forceinline__ int node_of(const TreeParams& p, int r) {
+  return p.group == 1 ? r : (int)__umulhi((uint32_t)r, p.group_inv);
+}
+
 // The wide kernel (tree_attn_tc.cu): its partials of a call, and the call itself. bf16, a
-// block size of a multiple of 16, a pool of under 2^31 rows.
+// block size of a multiple of 16, a pool of under 2^31 - 16 rows.
 size_t tree_attn_wide_partial_bytes(int batch, int max_q, int max_ctx, int nkv, int group, int hd);
 int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, cudaStream_t stream);
 

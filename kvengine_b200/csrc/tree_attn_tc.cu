@@ -4,14 +4,15 @@
 // rows (nodes x group heads) than the tile of m16 products can hide: the work is then
 // bound by the tensor cores and the exponentials rather than by the cache's bytes.
 //
-// A CTA has two softmax warpgroups, each with its own 128-row score tile S and output
+// A CTA has two softmax warpgroups, each with two 128-row score tiles S and one output
 // tile O in tensor memory, and one of two jobs:
 //   one query tile (up to 128 rows): the two groups take the even and the odd key tiles
 //     of the chunk, and their outputs are joined at the end;
 //   two query tiles (up to 256 rows): both groups take every key tile, one query tile
 //     each, so that a K/V tile is fetched into shared memory once for 256 rows.
-// Either way the tensor cores work on one group's tile while the other group is in its
-// softmax. Per key tile (128 keys) and group:
+// While a group is in the softmax of one tile, the tensor cores have its next S ready and
+// add its last P V: with 128-key tiles and one S a group, a step waited for both products
+// (4080 cycles a 128 keys, against 2300 in the softmax). Per key tile (64 keys) and group:
 //   S = Q K^T      tcgen05.mma, Q and K in shared memory (128-byte swizzle, K-major)
 //   P = 2^(S sl - m)  one thread a row: a pass for the maximum, a pass for the exponentials;
 //                  P goes back to tensor memory as bf16, over S
@@ -30,6 +31,7 @@
 
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include "kve_common.cuh"
 #include "tma.cuh"
@@ -38,10 +40,11 @@
 namespace kve {
 namespace {
 
-constexpr int kKeys = 128;       // keys of a tile
+constexpr int kKeys = 64;        // keys of a tile
 constexpr int kRows = 128;       // query rows of a tile
-constexpr int kThreads = 384;    // loader, MMA issuer, V warp, TMEM warp; two softmax warpgroups
-constexpr int kMaxSlots = 8;
+constexpr int kThreads = 384;    // loader, a warp of products for each group, V warp; two softmax warpgroups
+constexpr int kMaxSlots = 12;
+constexpr int kShare = 4;        // every kShare-th pair of exponentials runs on the fp32 units
 
 __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
@@ -56,38 +59,77 @@ __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t half_b
 __device__ __forceinline__ uint32_t mma_idesc(int n, bool b_mn) {
   return 1u << 4 | 1u << 7 | 1u << 10 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kRows >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
+// Products and commits are written for a whole warp that runs together, with one lane
+// issuing: their descriptors then stay in uniform registers (issued from a branch of
+// one lane, each product cost 75 to 100 cycles, more than it computes).
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accum), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accum), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t lead, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
+}
+// A TMA load by the warp's issuing lane, like the products: from lanes with coordinates of
+// their own, one box after the other, each cost about 140 cycles.
+__device__ __forceinline__ void tma_load(uint32_t lead, uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void tma_load_v(uint32_t lead, uint32_t dst, const CUtensorMap* map, int y, int z, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%6, %2, %3}], [%4];\n\t}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(y), "r"(z), "r"(bar), "r"(lead), "r"(0) : "memory");
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns of this thread's lane: asked for here, there after tmem_arrived on the same registers.
+__device__ __forceinline__ void tmem_ask(uint32_t addr, float (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_arrived(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+                 "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+                 "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
+                 "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :: "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+  tmem_ask(addr, v);
+  tmem_arrived(v);
 }
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const float (&v)[32]) {
   asm volatile(
@@ -111,6 +153,42 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[
       : "memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two fp32 operations in one.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+// 2^x of two numbers up to 2^7 without the special-function unit: x = n + r, n the nearest
+// integer (x + 1.5 2^23 has it in its low bits), 2^r on [-1/2, 1/2] by the polynomial of
+// degree 4 of least relative error (2.6e-6, found by weighted least squares), n added to
+// the exponent. Below 2^-126: 2^-126, which is nothing beside a row's largest term.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 big = make_float2(12582912.f, 12582912.f), neg = make_float2(-12582912.f, -12582912.f);
+  const float2 t = add2(x, big);
+  const float2 r = fma2(add2(t, neg), make_float2(-1.f, -1.f), x);
+  float2 y = fma2(r, make_float2(0.00957009941f, 0.00957009941f), make_float2(0.0559178703f, 0.0559178703f));
+  y = fma2(y, r, make_float2(0.240247443f, 0.240247443f));
+  y = fma2(y, r, make_float2(0.693121791f, 0.693121791f));
+  y = fma2(y, r, make_float2(0.999999285f, 0.999999285f));
+  y.x = __int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23));
+  y.y = __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23));
+  return y;
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
@@ -125,10 +203,11 @@ struct WideShape {
   static constexpr int QT = TWO ? 2 : 1;
   static constexpr int QBYTES = kRows * HD * 2;
   static constexpr int SLOT = kKeys * HD * 2;
-  static constexpr int NS = HD == 128 ? (TWO ? 5 : 6) : 8;
+  static constexpr int NS = HD == 128 && TWO ? 10 : 12;
   static constexpr int XROW = HD + 4;  // floats of a row of the joining area (in the ring)
-  static constexpr int BARS = (3 * kMaxSlots + 6) * 8;
+  static constexpr int BARS = (3 * kMaxSlots + 12) * 8;
   static constexpr size_t SMEM = 1024 + (size_t)QT * QBYTES + (size_t)NS * SLOT + BARS + 64;
+  static_assert(NS <= kMaxSlots, "ring");
   static_assert(NS * SLOT >= kRows * (XROW + 2) * 4, "joining area");
   static_assert(SMEM <= 232448, "shared memory");
 };
@@ -137,38 +216,23 @@ template <int HD, bool TWO>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeParams p) {
   using W = WideShape<HD, TWO>;
-  constexpr int NS = W::NS, HALVES = HD / 64;
+  constexpr int NS = W::NS;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = smem;
   uint8_t* ring = smem + W::QT * W::QBYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + (size_t)NS * W::SLOT);
   uint64_t* full = bars;                     // a slot's TMA bytes have landed
-  uint64_t* ready = bars + kMaxSlots;        // by V tile (mod NS): the V warp has been over it
+  uint64_t* ready = bars + kMaxSlots;        // by special V tile (mod NK): the V warp has been over it
   uint64_t* empty = bars + 2 * kMaxSlots;    // the products that read it are done
-  uint64_t* s_ready = bars + 3 * kMaxSlots;  // by group: S is complete
-  uint64_t* p_ready = s_ready + 2;           // P is in tensor memory (one arrival a warp)
-  uint64_t* o_ready = s_ready + 4;           // O is complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kMaxSlots + 6);
+  uint64_t* s_ready = bars + 3 * kMaxSlots;  // by group and S buffer: S is complete
+  uint64_t* p_ready = s_ready + 4;           // likewise: P is in tensor memory (one arrival a warp)
+  uint64_t* pv_done = s_ready + 8;           // by group: its last P V is in O
+  uint64_t* o_ready = s_ready + 10;          // by group: O is complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kMaxSlots + 12);
   int* odd = reinterpret_cast<int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < NS; ++i) {
-      mbar_init(smem_u32(&full[i]), 1);
-      mbar_init(smem_u32(&ready[i]), 1);
-      mbar_init(smem_u32(&empty[i]), 1);
-    }
-    for (int g = 0; g < 2; ++g) {
-      mbar_init(smem_u32(&s_ready[g]), 1);
-      mbar_init(smem_u32(&p_ready[g]), 4);
-      mbar_init(smem_u32(&o_ready[g]), 1);
-    }
-    *odd = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    prefetch_map(&map_k);
-    prefetch_map(&map_v);
-  }
   grid_dep_wait();
   grid_dep_launch();
 
@@ -194,9 +258,35 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const int steps0 = TWO ? n : (n + 1) / 2, steps1 = TWO ? (rows > kRows ? n : 0) : n / 2;
   auto steps = [&](int g) { return g ? steps1 : steps0; };
   auto tile_of = [&](int g, int i) { return TWO ? i : 2 * i + g; };
-  // The ring's order is the order of use. TWO: K0 V0 K1 V1 ..; else K0 K1 V0 K2 V1 .. V(n-2) V(n-1).
-  auto k_item = [&](int t) { return TWO ? 2 * t : t < 2 ? t : 2 * t - 1; };
-  auto v_item = [&](int t) { return TWO ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1); };
+  // Tiles from here on have keys that are new tokens or lie behind the last key.
+  const int special = max(0, min(hist - key_lo, key_hi - key_lo)) / kKeys;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(smem_u32(&full[i]), 1);
+      mbar_init(smem_u32(&ready[i]), 1);
+      mbar_init(smem_u32(&empty[i]), TWO && steps1 > 0 ? 2 : 1);  // one commit of each group that reads it
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(smem_u32(&s_ready[2 * g]), 1);
+      mbar_init(smem_u32(&s_ready[2 * g + 1]), 1);
+      mbar_init(smem_u32(&p_ready[2 * g]), 4);
+      mbar_init(smem_u32(&p_ready[2 * g + 1]), 4);
+      mbar_init(smem_u32(&pv_done[g]), 1);
+      mbar_init(smem_u32(&o_ready[g]), 1);
+    }
+    *odd = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+  }
+  __syncthreads();  // the barriers are there: the copies may start
+  // K tile t lies in slot t mod NK, V tile t in slot NK + t mod NK; each slot has its barriers.
+  constexpr int NK = NS / 2;
+  auto slot_of = [&](bool v, int t) { return (v ? NK : 0) + t % NK; };
+  auto slot_addr = [&](bool v, int t) { return smem_u32(ring) + (uint32_t)(slot_of(v, t) * W::SLOT); };
+  auto parity_of = [&](int t) { return (uint32_t)(t / NK) & 1u; };
+  bool ok = true;  // no wait of this thread has run out
 
   if (warp == 3) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
@@ -204,241 +294,281 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   }
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q);
   auto head_row = [&](int r) {  // row r of the CTA in q and out
-    const int gr = row0 + r;
-    return ((size_t)(qoff + gr / p.group) * p.nq + h * p.group + gr % p.group) * HD;
+    const int gr = row0 + r, node = node_of(p, gr);
+    return ((size_t)(qoff + node) * p.nq + h * p.group + gr - node * p.group) * HD;
   };
   if (warp >= 4) {
     // Q into shared memory, 16 bytes a lane; a negative scale is a sign on q.
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-    for (int i = threadIdx.x - 128; i < W::QT * kRows * (HD / 8); i += 256) {
-      const int r = i / (HD / 8), ch = i % (HD / 8);
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows) x = *reinterpret_cast<const uint4*>(q + head_row(r) + ch * 8);
-      x.x ^= flip;
-      x.y ^= flip;
-      x.z ^= flip;
-      x.w ^= flip;
-      const int rr = r % kRows;
-      uint8_t* dst = q_smem + (r / kRows) * W::QBYTES + (ch / 8) * (kRows * 128) + rr * 128 + (((ch % 8) ^ (rr & 7)) << 4);
-      *reinterpret_cast<uint4*>(dst) = x;
+    // TWO: each group its own tile; else half of the one
+    constexpr int PER = kRows * (HD / 8) / (TWO ? 128 : 256);
+    const int first = TWO ? threadIdx.x & 127 : threadIdx.x - 128, tile = TWO ? (threadIdx.x - 128) / 128 : 0;
+    uint4 x[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int i = first + u * (TWO ? 128 : 256), r = tile * kRows + i / (HD / 8);
+      x[u] = r < rows ? *reinterpret_cast<const uint4*>(q + head_row(r) + i % (HD / 8) * 8) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int i = first + u * (TWO ? 128 : 256), r = i / (HD / 8), ch = i % (HD / 8);
+      x[u].x ^= flip;
+      x[u].y ^= flip;
+      x[u].z ^= flip;
+      x[u].w ^= flip;
+      *reinterpret_cast<uint4*>(q_smem + tile * W::QBYTES + (ch / 8) * (kRows * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4)) = x[u];
     }
     fence_proxy_async_smem();
   }
-  tc_before();
-  __syncthreads();
-  tc_after();
-  const uint32_t tmem = *tmem_slot;
-  auto s_col = [&](int g) { return tmem + (uint32_t)(g * 128); };
+  uint32_t tmem = 0;
+  if (warp != 0) {  // Q and tensor memory are there
+    tc_before();
+    asm volatile("bar.sync 2, 352;" ::: "memory");
+    tc_after();
+    tmem = *tmem_slot;
+  }
+  auto s_col = [&](int g, int i) { return tmem + (uint32_t)(g * 128 + (i & 1) * kKeys); };
   auto o_col = [&](int g) { return tmem + (uint32_t)(256 + g * 128); };
-  auto slot_addr = [&](int item) { return smem_u32(ring) + (uint32_t)((item % NS) * W::SLOT); };
-  bool ok = true;  // no wait of this thread has run out
-  const int items = 2 * n;
 
   float m = -INFINITY, l = 0.f;  // softmax threads: the row's base and its sum
   const int grp = warp >= 8 ? 1 : 0, row = (warp & 3) * 32 + lane;
+  // The first pool rows of the tiles' groups of 16 keys, lane l knowing group 32 w + l (past the end: a
+  // row behind the pool, which loads as zeros).
+  auto rows_of = [&](int w, bool tell) {
+    const int key = key_lo + (w * 32 + lane) * 16;
+    int y = (int)(p.num_blocks * p.bs);
+    if (key < key_hi) {
+      const int blk = p.tables[(size_t)b * p.table_stride + key / p.bs];
+      if (blk >= 0 && blk < p.num_blocks) y = blk * p.bs + key % p.bs;
+      else if (tell) report(p.status, KVE_ERR_BOUNDS);
+    }
+    return y;
+  };
   if (warp == 0) {
-    // ---- loader: lanes 0 .. 7 ask for 16 keys each
-    const int32_t* table = p.tables + (size_t)b * p.table_stride;
-    const int past = (int)(p.num_blocks * p.bs);  // rows from here on load as zeros
-    auto load = [&](const CUtensorMap* map, int t, int item) {
-      const int slot = item % NS;
-      if (item >= NS) ok = ok && mbar_wait(smem_u32(&empty[slot]), (uint32_t)(item / NS - 1) & 1u, p.status);
+    // ---- K: boxes of 16 keys x 64 dims
+    const uint32_t lead = elect_lane();
+    int now = rows_of(0, true), next = rows_of(1, true);
+    for (int t = 0; t < n; ++t) {
+      if (t > 0 && t % 8 == 0) {
+        now = next;
+        next = rows_of(t / 8 + 1, true);
+      }
+      const uint32_t bar = smem_u32(&full[slot_of(false, t)]);
+      if (t >= NK) ok = ok && mbar_wait(smem_u32(&empty[slot_of(false, t)]), parity_of(t - NK), p.status);
       ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        for (int u = t - NK; u < t; ++u) mbar_wait(smem_u32(&full[slot_of(false, u)]), parity_of(u), p.status);  // in flight
+        break;
+      }
+      if (lead) mbar_expect_tx(bar, W::SLOT);
+      __syncwarp();
+#pragma unroll
+      for (int part = 0; part < kKeys / 16; ++part) {
+        const int y = __shfl_sync(0xffffffffu, now, t % 8 * 4 + part);
+#pragma unroll
+        for (int half = 0; half < HD / 64; ++half)
+          tma_load(lead, slot_addr(false, t) + half * (kKeys * 128) + part * 2048, &map_k, h * HD + half * 64, y, bar);
+      }
+    }
+  } else if (warp <= 2) {
+    // ---- products of one group. (One warp for both took 2350 cycles a step with its waits, whatever
+    // the products and the softmax cost.)
+    const int g = warp - 1, my_steps = steps(g);
+    const uint32_t lead = elect_lane();
+    const uint32_t id_qk = mma_idesc(kKeys, false), id_pv = mma_idesc(HD, true);
+    const uint64_t ad = desc_k_major(smem_u32(q_smem) + (TWO ? g * W::QBYTES : 0));
+    auto qk = [&](int i) {
+      const int t = tile_of(g, i), slot = slot_of(false, t);
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&full[slot]), parity_of(t), p.status));
       if (!ok) return;
-      if (lane == 0) mbar_expect_tx(smem_u32(&full[slot]), W::SLOT);
-      __syncwarp();
-      if (lane < 8) {
-        const int key = key_lo + t * kKeys + lane * 16;
-        int y = past;
-        if (key < key_hi) {
-          const int blk = table[key / p.bs];
-          if (blk >= 0 && blk < p.num_blocks) y = (int)((int64_t)blk * p.bs + key % p.bs);
-          else report(p.status, KVE_ERR_BOUNDS);
-        }
+      tc_after();
+      const uint64_t bd = desc_k_major(slot_addr(false, t));
 #pragma unroll
-        for (int half = 0; half < HALVES; ++half)
-          tma_load_2d(slot_addr(item) + half * (kKeys * 128) + lane * 2048, map, h * HD + half * 64, y, smem_u32(&full[slot]));
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        const uint64_t a_step = (uint64_t)((kk / 4) * (kRows * 128 / 16) + (kk % 4) * 2);
+        const uint64_t b_step = (uint64_t)((kk / 4) * (kKeys * 128 / 16) + (kk % 4) * 2);
+        mma_ss(lead, s_col(g, i), ad + a_step, bd + b_step, id_qk, kk > 0);
       }
-      __syncwarp();
+      mma_commit(lead, smem_u32(&empty[slot]));
+      mma_commit(lead, smem_u32(&s_ready[2 * g + (i & 1)]));
     };
-    int done = 0;
-    for (int item = 0; item < items && ok; ++item) {
-      // which tile's K or V comes next
-      int t;
-      bool is_k;
-      if (TWO) {
-        t = item / 2;
-        is_k = item % 2 == 0;
-      } else if (item < 2) {
-        t = n == 1 ? 0 : item;
-        is_k = n > 1 || item == 0;
-      } else {
-        is_k = item % 2 == 1 && item != items - 1;
-        t = is_k ? (item + 1) / 2 : item == items - 1 ? n - 1 : item / 2 - 1;
-      }
-      load(is_k ? &map_k : &map_v, t, item);
-      done = item + 1;
-    }
-    if (!ok)  // let what is in flight land
-      for (int item = max(0, done - NS); item < done; ++item)
-        mbar_wait(smem_u32(&full[item % NS]), (uint32_t)(item / NS) & 1u, p.status);
-  } else if (warp == 1) {
-    // ---- MMA issuer
-    if (lane == 0) {
-      const uint32_t id_qk = mma_idesc(kKeys, false), id_pv = mma_idesc(HD, true);
-      const int last_user = TWO ? (steps1 ? 1 : 0) : -1;  // TWO: the group whose product is a slot's last
-      auto qk = [&](int g, int i) {
-        const int item = k_item(tile_of(g, i)), slot = item % NS;
-        ok = ok && mbar_wait(smem_u32(&full[slot]), (uint32_t)(item / NS) & 1u, p.status);
-        if (!ok) return;
-        tc_after();
-        const uint64_t ad = desc_k_major(smem_u32(q_smem) + (TWO ? g * W::QBYTES : 0)), bd = desc_k_major(slot_addr(item));
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint64_t step = (uint64_t)((kk / 4) * (kKeys * 128 / 16) + (kk % 4) * 2);
-          mma_ss(s_col(g), ad + step, bd + step, id_qk, kk > 0);
-        }
-        if (!TWO || g == last_user) mma_commit(smem_u32(&empty[slot]));
-        mma_commit(smem_u32(&s_ready[g]));
-      };
-      auto pv = [&](int g, int i) {
-        const int t = tile_of(g, i), item = v_item(t), slot = item % NS;
-        ok = ok && mbar_wait(smem_u32(&p_ready[g]), (uint32_t)i & 1u, p.status);
-        ok = ok && mbar_wait(smem_u32(&full[slot]), (uint32_t)(item / NS) & 1u, p.status);
-        ok = ok && mbar_wait(smem_u32(&ready[t % NS]), (uint32_t)(t / NS) & 1u, p.status);
-        if (!ok) return;
-        tc_after();
-        const uint64_t bd = desc_mn_major(slot_addr(item), kKeys * 128);
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          mma_ts(o_col(g), s_col(g) + kk * 8, bd + (uint64_t)(kk * (2048 / 16)), id_pv, i > 0 || kk > 0);
-        if (!TWO || g == last_user) mma_commit(smem_u32(&empty[slot]));
-      };
-      for (int g = 0; g < 2; ++g)
-        if (steps(g) > 0) qk(g, 0);
-      for (int i = 0; i < steps0 && ok; ++i)
-        for (int g = 0; g < 2; ++g) {
-          if (i >= steps(g)) continue;
-          pv(g, i);
-          if (i + 1 < steps(g)) qk(g, i + 1);
-          else mma_commit(smem_u32(&o_ready[g]));
-        }
-      if (!ok) {  // end what was issued before the memory it uses goes away
-        mma_commit(smem_u32(&o_ready[0]));
-        mbar_wait(smem_u32(&o_ready[0]), 0, p.status);
-      }
-    }
-    __syncwarp();
-  } else if (warp == 2) {
-    // ---- V: zero rows behind the last key, look for infinities and NaN in new tokens' rows
-    for (int t = 0; t < n && ok; ++t) {
-      const int item = v_item(t), slot = item % NS;
-      ok = ok && mbar_wait(smem_u32(&full[slot]), (uint32_t)(item / NS) & 1u, p.status);
+    for (int i = 0; i < 2 && i < my_steps && ok; ++i) qk(i);
+    for (int i = 0; i < my_steps && ok; ++i) {
+      const int t = tile_of(g, i), slot = slot_of(true, t);
+      ok = t >= special ? mbar_wait(smem_u32(&ready[(t - special) % NK]), parity_of(t - special), p.status)
+                        : mbar_wait(smem_u32(&full[slot]), parity_of(t), p.status);
+      ok = ok && mbar_wait(smem_u32(&p_ready[2 * g + (i & 1)]), (uint32_t)(i / 2) & 1u, p.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      tc_after();
+      const uint64_t bd = desc_mn_major(slot_addr(true, t), 2048);
+#pragma unroll
+      for (int kk = 0; kk < kKeys / 16; ++kk)
+        mma_ts(lead, o_col(g), s_col(g, i) + kk * 8, bd + (uint64_t)(kk * (16 * HD * 2 / 16)), id_pv, i > 0 || kk > 0);
+      mma_commit(lead, smem_u32(&empty[slot]));
+      mma_commit(lead, smem_u32(&pv_done[g]));
+      if (i + 1 == my_steps) mma_commit(lead, smem_u32(&o_ready[g]));
+      else if (i + 2 < my_steps) qk(i + 2);
+    }
+    if (!ok) {  // end what was issued before the memory it uses goes away
+      mma_commit(lead, smem_u32(&o_ready[g]));
+      mbar_wait(smem_u32(&o_ready[g]), 0, p.status);
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ---- V: boxes of 16 keys x all dims (a product takes 16 keys: their halves may lie 2 KB apart).
+    // Special tiles: zero the rows behind the last key, look for infinities and NaN in new tokens' rows.
+    auto look = [&](int t) {
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&full[slot_of(true, t)]), parity_of(t), p.status));
+      if (!ok) return;
       const int kt = key_lo + t * kKeys;
-      uint8_t* v = ring + (size_t)slot * W::SLOT;
+      uint8_t* v = ring + (size_t)slot_of(true, t) * W::SLOT;
+      auto piece = [&](int r, int i) {  // 16 bytes i of row r, in any order
+        return reinterpret_cast<uint4*>(v + (r / 16) * (16 * HD * 2) + (i / 8) * 2048 + (r % 16) * 128 + i % 8 * 16);
+      };
+      constexpr int PIECES = HD / 8;
       if (kt + kKeys > key_hi) {
         const int first = key_hi - kt, stop = min(kKeys, (first + 15) / 16 * 16);  // further boxes are zeros already
-        for (int i = lane; i < (stop - first) * 8 * HALVES; i += 32) {
-          const int half = i / ((stop - first) * 8), rem = i % ((stop - first) * 8);
-          *reinterpret_cast<uint4*>(v + half * (kKeys * 128) + (first + rem / 8) * 128 + rem % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int i = lane; i < (stop - first) * PIECES; i += 32) *piece(first + i / PIECES, i % PIECES) = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
       }
       const int r0 = max(hist - kt, 0), r1 = min(kKeys, key_hi - kt);
-      if (r0 < r1) {
-        bool found = false;
-        for (int i = lane; i < (r1 - r0) * 8 * HALVES; i += 32) {
-          const int half = i / ((r1 - r0) * 8), rem = i % ((r1 - r0) * 8);
-          const uint4 x = *reinterpret_cast<const uint4*>(v + half * (kKeys * 128) + (r0 + rem / 8) * 128 + rem % 8 * 16);
-          found |= odd_bits(x.x) || odd_bits(x.y) || odd_bits(x.z) || odd_bits(x.w);
-        }
-        if (__any_sync(0xffffffffu, found) && lane == 0) *odd = 1;
+      bool found = false;
+      for (int i = lane; i < (r1 - r0) * PIECES; i += 32) {
+        const uint4 x = *piece(r0 + i / PIECES, i % PIECES);
+        found |= odd_bits(x.x) || odd_bits(x.y) || odd_bits(x.z) || odd_bits(x.w);
       }
+      if (__any_sync(0xffffffffu, found) && lane == 0) *odd = 1;
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ready[t % NS]));
+      if (lane == 0) mbar_arrive(smem_u32(&ready[(t - special) % NK]));
+    };
+    const uint32_t lead = elect_lane();
+    int now = rows_of(0, false), next = rows_of(1, false), looked = special;
+    for (int t = 0; t < n; ++t) {
+      if (t > 0 && t % 8 == 0) {
+        now = next;
+        next = rows_of(t / 8 + 1, false);
+      }
+      const uint32_t bar = smem_u32(&full[slot_of(true, t)]);
+      while (ok && looked <= t - NK) look(looked++);  // their products free the slots
+      if (t >= NK) ok = ok && mbar_wait(smem_u32(&empty[slot_of(true, t)]), parity_of(t - NK), p.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        for (int u = max(0, t - NK); u < t; ++u) mbar_wait(smem_u32(&full[slot_of(true, u)]), parity_of(u), p.status);
+        break;
+      }
+      if (lead) mbar_expect_tx(bar, W::SLOT);
+      __syncwarp();
+#pragma unroll
+      for (int part = 0; part < kKeys / 16; ++part) {
+        const int y = __shfl_sync(0xffffffffu, now, t % 8 * 4 + part);
+        tma_load_v(lead, slot_addr(true, t) + part * (16 * HD * 2), &map_v, y, h * (HD / 64), bar);
+      }
+      if (looked < t && __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&full[slot_of(true, looked)]), parity_of(looked))))
+        look(looked++);
     }
+    while (ok && looked < n) look(looked++);
   } else if (warp >= 4) {
     // ---- softmax: a thread a row
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int r = (TWO ? grp * kRows : 0) + row;  // row of the CTA
     const bool active = (TWO ? grp * kRows : 0) + (warp & 3) * 32 < rows;  // any row of this warp
-    const int node = (row0 + min(r, rows - 1)) / p.group;
+    const int node = node_of(p, row0 + min(r, rows - 1));
     const uint32_t* mask = p.mask ? p.mask + (size_t)(qoff + node) * p.mask_words : nullptr;
     const float sl = fabsf(p.scale) * 1.4426950408889634f;
     const int my_steps = steps(grp);
+    // One tile: m and l, and P over S. `masked`: some of the tile's keys are new tokens or
+    // lie behind the last key.
+    auto softmax_step = [&](int i, int kt, auto masked) {
+      const uint32_t sc = s_col(grp, i) + lanes;
+      uint32_t see[kKeys / 32];
+      if constexpr (masked) {
+#pragma unroll
+        for (int w = 0; w < kKeys / 32; ++w) {
+          const int at = kt + 32 * w;
+          see[w] = p.mask ? mask_bits<32>(mask, p.mask_words, at - hist) : chain_bits(node, at - hist);
+          const int in = key_hi - at;
+          see[w] &= in >= 32 ? ~0u : in <= 0 ? 0u : (1u << in) - 1u;
+        }
+      }
+      float v[kKeys / 32][32];  // the row of S stays in registers
+#pragma unroll
+      for (int w = 0; w < kKeys / 32; ++w) tmem_ask(sc + 32 * w, v[w]);
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kKeys / 32; ++w) {
+        tmem_arrived(v[w]);
+        if constexpr (masked) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[w][j] = see[w] >> j & 1 ? v[w][j] : -INFINITY;
+        }
+        float part[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          part[j] = max3(v[w][j], v[w][j + 4], v[w][j + 8]);
+          part[j] = max3(part[j], v[w][j + 12], v[w][j + 16]);
+          part[j] = max3(part[j], v[w][j + 20], v[w][j + 24]);
+          part[j] = fmaxf(part[j], v[w][j + 28]);
+        }
+        top = max3(top, max3(part[0], part[1], part[2]), part[3]);
+      }
+      top *= sl;  // 0 x infinity: NaN, and no new base
+      const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow ? ex2(m - top) : 1.f;
+        if (grow) m = top;
+        l *= f;
+        if (i > 0) {
+          ok = ok && mbar_wait(smem_u32(&pv_done[grp]), (uint32_t)(i - 1) & 1u, p.status);  // O is not being added to
+          __syncwarp();
+          tc_after();
+#pragma unroll 1
+          for (int w = 0; w < HD / 32; ++w) {
+            float o[32];
+            tmem_load(o_col(grp) + lanes + 32 * w, o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] *= f;
+            tmem_store32(o_col(grp) + lanes + 32 * w, o);
+          }
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : -m;
+      const float2 sl2 = make_float2(sl, sl), off2 = make_float2(off, off);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int w = 0; w < kKeys / 32; ++w) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float2 e = fma2(make_float2(v[w][2 * j], v[w][2 * j + 1]), sl2, off2);
+          if (!masked && j % kShare == kShare - 1) {
+            e = ex2_fma(e);
+          } else {
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+          }
+          sum[j & 1] = add2(sum[j & 1], e);
+          packed[j] = pack2(e.x, e.y);
+        }
+        tmem_store16(sc + 16 * w, packed);  // over S
+      }
+      sum[0] = add2(sum[0], sum[1]);
+      l += sum[0].x + sum[0].y;
+    };
     for (int i = 0; i < my_steps; ++i) {
-      ok = ok && mbar_wait(smem_u32(&s_ready[grp]), (uint32_t)i & 1u, p.status);
+      ok = ok && mbar_wait(smem_u32(&s_ready[2 * grp + (i & 1)]), (uint32_t)(i / 2) & 1u, p.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (active) {
         tc_after();
         const int kt = key_lo + tile_of(grp, i) * kKeys;
-        const bool masked = kt + kKeys > hist || kt + kKeys > key_hi;
-        uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
-        if (masked) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int at = kt + 32 * w;
-            see[w] = p.mask ? mask_bits<32>(mask, p.mask_words, at - hist) : chain_bits(node, at - hist);
-            const int in = key_hi - at;
-            see[w] &= in >= 32 ? ~0u : in <= 0 ? 0u : (1u << in) - 1u;
-          }
-        }
-        const uint32_t sc = s_col(grp) + lanes;
-        float top = -INFINITY;
-        float v[32];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          tmem_load(sc + 32 * w, v);
-          if (masked) {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) top = fmaxf(top, see[w] >> x & 1 ? v[x] : -INFINITY);
-          } else {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) top = fmaxf(top, v[x]);
-          }
-        }
-        top *= sl;  // 0 x infinity: NaN, and no new base
-        const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float f = grow ? ex2(m - top) : 1.f;
-          if (grow) m = top;
-          l *= f;
-          if (i > 0) {
-#pragma unroll 1
-            for (int w = 0; w < HD / 32; ++w) {
-              tmem_load(o_col(grp) + lanes + 32 * w, v);
-#pragma unroll
-              for (int x = 0; x < 32; ++x) v[x] *= f;
-              tmem_store32(o_col(grp) + lanes + 32 * w, v);
-            }
-          }
-        }
-        const float off = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          tmem_load(sc + 32 * w, v);
-          uint32_t packed[16];
-#pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            float e = fmaf(v[x], sl, off);
-            if (masked) e = see[w] >> x & 1 ? e : -INFINITY;
-            v[x] = ex2(e);
-            sum[x & 3] += v[x];
-          }
-#pragma unroll
-          for (int x = 0; x < 16; ++x) packed[x] = pack2(v[2 * x], v[2 * x + 1]);
-          tmem_store16(sc + 16 * w, packed);  // over columns of S already read
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (kt + kKeys > hist || kt + kKeys > key_hi) softmax_step(i, kt, std::true_type());
+        else softmax_step(i, kt, std::false_type());
         tmem_store_wait();
       }
       tc_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&p_ready[grp]));
+      if (lane == 0) mbar_arrive(smem_u32(&p_ready[2 * grp + (i & 1)]));
     }
     if (my_steps > 0) ok = ok && mbar_wait(smem_u32(&o_ready[grp]), 0, p.status);
     tc_after();
@@ -499,8 +629,9 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
               v[x + 3] = v[x + 3] * f0 + y.w * f1;
             }
           }
-          if (r < rows && live == 1) {
-            __nv_bfloat16* dst = out + head_row(r) + 32 * w;
+          if (live == 1) {
+            // to shared memory (Q is no longer needed), 16-byte pieces exchanged by row
+            uint8_t* dst = q_smem + (size_t)r * (HD * 2);
 #pragma unroll
             for (int x = 0; x < 32; x += 8) {
               uint4 o;
@@ -508,7 +639,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
               o.y = pack2(l == 0.f ? 0.f : v[x + 2] * inv, l == 0.f ? 0.f : v[x + 3] * inv);
               o.z = pack2(l == 0.f ? 0.f : v[x + 4] * inv, l == 0.f ? 0.f : v[x + 5] * inv);
               o.w = pack2(l == 0.f ? 0.f : v[x + 6] * inv, l == 0.f ? 0.f : v[x + 7] * inv);
-              *reinterpret_cast<uint4*>(dst + x) = o;
+              *reinterpret_cast<uint4*>(dst + (((w * 4 + x / 8) ^ (r & 7)) << 4)) = o;
             }
           } else if (r < rows) {
             float* dst = part + (size_t)r * PROW + 32 * w;
@@ -519,6 +650,18 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
           __syncwarp();  // the loads of tensor memory are the whole warp's
         }
         if (live > 1 && r < rows) *reinterpret_cast<float2*>(part + (size_t)r * PROW + HD) = make_float2(m, l);
+        if (live == 1) {
+          // this warp's 32 rows, whole rows at a time
+          const int r0 = (TWO ? grp * kRows : 0) + (warp & 3) * 32;
+          constexpr int PIECES = HD / 8, AT_ONCE = 32 / PIECES;
+#pragma unroll 4
+          for (int rr = lane / PIECES; rr < 32; rr += AT_ONCE) {
+            const int ro = r0 + rr, piece = lane % PIECES;
+            if (ro < rows)
+              *reinterpret_cast<uint4*>(out + head_row(ro) + piece * 8) =
+                  *reinterpret_cast<const uint4*>(q_smem + (size_t)ro * (HD * 2) + ((piece ^ (ro & 7)) << 4));
+          }
+        }
       }
     }
   }
@@ -530,7 +673,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const __nv_bfloat16* pv = static_cast<const __nv_bfloat16*>(p.pool_v);
     const float sl = p.scale * 1.4426950408889634f;
     for (int r = warp; r < rows; r += kThreads / 32) {
-      const int node = (row0 + r) / p.group;
+      const int node = node_of(p, row0 + r);
       const uint32_t* mask = p.mask ? p.mask + (size_t)(qoff + node) * p.mask_words : nullptr;
       float qv[DPL], acc[DPL] = {};
 #pragma unroll
@@ -617,7 +760,7 @@ struct WidePlan {
 
 // One or two query tiles a CTA by the rows of the call's largest tree, and the number
 // of chunks that costs least: waves of one CTA an SM, each a fixed part (launch, Q,
-// the first tile's latency, joining: about 5 us) and a part per step (about 1.4 us).
+// the first tile's latency, joining: about 5 us) and a part per step (about 0.7 us).
 WidePlan wide_plan(int batch, int max_q, int max_ctx, int nkv, int group) {
   WidePlan w;
   const long long rows = (long long)max_q * group;
@@ -634,7 +777,7 @@ WidePlan wide_plan(int batch, int max_q, int max_ctx, int nkv, int group) {
     if (chunks != c || (c > 1 && units > (long long)kTreeCounterSlots)) continue;
     const int steps = w.two ? per_chunk : (per_chunk + 1) / 2;
     const double waves = (double)((units * c + 147) / 148);
-    const double t = waves * (5.0 + 1.4 * steps) + (c > 1 ? 2.0 + 0.15 * c : 0.0);
+    const double t = waves * (5.0 + 0.7 * steps) + (c > 1 ? 2.0 + 0.15 * c : 0.0);
     if (t < best) {
       best = t;
       w.chunk = per_chunk * kKeys;
@@ -644,15 +787,18 @@ WidePlan wide_plan(int batch, int max_q, int max_ctx, int nkv, int group) {
   return w;
 }
 
-bool pool_map(CUtensorMap* map, const void* pool, int64_t rows, int width) {
+// One layer's pool as (64 dims, rows) with boxes of 16 rows, and, for V, as (64 dims, rows, dims / 64)
+// with boxes of 16 rows and all of a head's dims.
+bool pool_map(CUtensorMap* map, const void* pool, int64_t rows, int width, int hd, bool v) {
   EncodeTiledFn fn = encode_fn();
   if (!fn || width >= (1 << 24)) return false;
-  return cached_map(map, pool, (uint64_t)rows | (uint64_t)width << 32, [&](CUtensorMap* m) {
-    cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)width * 2};
-    cuuint32_t box[2] = {64, 16};
-    cuuint32_t estr[2] = {1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, estr,
+  return cached_map(map, pool, (uint64_t)rows | (uint64_t)width << 32 | (uint64_t)(v ? hd : 0) << 56, [&](CUtensorMap* m) {
+    cuuint64_t dims2[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    cuuint64_t dims3[3] = {64, (cuuint64_t)rows, (cuuint64_t)width / 64};
+    cuuint64_t strides[2] = {(cuuint64_t)width * 2, 128};
+    cuuint32_t box[3] = {64, 16, (cuuint32_t)hd / 64};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v ? 3 : 2, const_cast<void*>(pool), v ? dims3 : dims2, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   });
@@ -695,7 +841,7 @@ int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, cudaStream_t st
   memset(&mk, 0, sizeof(mk));
   memset(&mv, 0, sizeof(mv));
   const int64_t rows = p.num_blocks * p.bs;
-  if (!pool_map(&mk, p.pool_k, rows, p.nkv * hd) || !pool_map(&mv, p.pool_v, rows, p.nkv * hd))
+  if (!pool_map(&mk, p.pool_k, rows, p.nkv * hd, hd, false) || !pool_map(&mv, p.pool_v, rows, p.nkv * hd, hd, true))
     return set_error(KVE_ERR_CUDA, "kve_paged_tree_attn: no tensor map for the pool");
   if (hd == 64) return w.two ? launch<64, true>(p, mk, mv, batch, stream) : launch<64, false>(p, mk, mv, batch, stream);
   return w.two ? launch<128, true>(p, mk, mv, batch, stream) : launch<128, false>(p, mk, mv, batch, stream);
