@@ -794,6 +794,8 @@ extern "C" size_t kve_tree_attn_workspace_bytes(int batch, int max_q_len, int ma
     const size_t w = tree_attn_wide_partial_bytes(batch, max_q_len, max_ctx, num_kv_heads, num_heads / num_kv_heads, head_dim);
     n = n > w ? n : w;
   }
+  const size_t few = tree_attn_small_partial_bytes(batch, max_ctx, num_kv_heads, head_dim);
+  n = n > few ? n : few;
   return n ? kTreeCounterBytes + n : 0;
 }
 
@@ -826,14 +828,6 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
     return set_error(KVE_ERR_ARG, "%s: %d mask words for %d nodes", me, mask_words, max_q_len);
   if ((uintptr_t)pool_k % 16 || (uintptr_t)pool_v % 16 || (uintptr_t)q % 16 || (uintptr_t)out % 16)
     return set_error(KVE_ERR_ARG, "%s: q, out and the pools must be 16-byte aligned", me);
-  const Split s = split_of(batch, max_q_len, max_ctx, num_kv_heads, group);
-  const bool wide = kv_dtype == KVE_BF16 && use_wide(max_q_len, group) && block_size % 16 == 0 &&
-                    num_blocks * block_size < 0x7ffffff0LL;
-  const size_t part = wide ? tree_attn_wide_partial_bytes(batch, max_q_len, max_ctx, num_kv_heads, group, head_dim)
-                           : partial_bytes(s, batch, num_kv_heads, head_dim);
-  if (part && (!workspace || workspace_bytes < kTreeCounterBytes + part))
-    return set_error(KVE_ERR_WORKSPACE, "%s: workspace needs %zu bytes", me, kTreeCounterBytes + part);
-  if (part && (uintptr_t)workspace % 16) return set_error(KVE_ERR_ARG, "%s: workspace must be 16-byte aligned", me);
   TreeParams p{};
   p.q = q; p.pool_k = pool_k; p.pool_v = pool_v; p.k_scale = k_scale; p.v_scale = v_scale;
   p.tables = block_tables; p.table_stride = table_stride;
@@ -841,12 +835,24 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
   p.mask = tree_mask; p.mask_words = mask_words;
   p.max_q = max_q_len; p.nq = num_heads; p.nkv = num_kv_heads; p.group = group; p.bs = block_size;
   p.group_inv = (uint32_t)((1ull << 32) / (uint32_t)group + 1);
-  p.num_blocks = num_blocks; p.scale = scale; p.out = out;
+  p.num_blocks = num_blocks; p.scale = scale; p.out = out; p.status = dev_status;
+  const bool fp8 = kv_dtype == KVE_FP8_E4M3;
+  const Split s = split_of(batch, max_q_len, max_ctx, num_kv_heads, group);
+  const bool small = dtype == KVE_BF16 && tree_attn_small_takes(p, fp8);
+  const bool wide = !small && kv_dtype == KVE_BF16 && use_wide(max_q_len, group) && block_size % 16 == 0 &&
+                    num_blocks * block_size < 0x7ffffff0LL;
+  const size_t part = small  ? tree_attn_small_partial_bytes(batch, max_ctx, num_kv_heads, head_dim)
+                      : wide ? tree_attn_wide_partial_bytes(batch, max_q_len, max_ctx, num_kv_heads, group, head_dim)
+                             : partial_bytes(s, batch, num_kv_heads, head_dim);
+  if (part && (!workspace || workspace_bytes < kTreeCounterBytes + part))
+    return set_error(KVE_ERR_WORKSPACE, "%s: workspace needs %zu bytes", me, kTreeCounterBytes + part);
+  if (part && (uintptr_t)workspace % 16) return set_error(KVE_ERR_ARG, "%s: workspace must be 16-byte aligned", me);
   p.counters = static_cast<int*>(workspace);
   p.partials = part ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kTreeCounterBytes) : nullptr;
-  p.chunk = s.chunk; p.n_chunks = s.n_chunks; p.n_qtiles = s.n_qtiles; p.status = dev_status;
+  p.chunk = s.chunk; p.n_chunks = s.n_chunks; p.n_qtiles = s.n_qtiles;
+  if (small) return tree_attn_small(p, batch, max_ctx, head_dim, fp8, stream);
   if (wide) return tree_attn_wide(p, batch, max_ctx, head_dim, stream);
-  if (kv_dtype == KVE_FP8_E4M3) return launch_hd<kFp8>(p, head_dim, s.rb, batch, stream);
+  if (fp8) return launch_hd<kFp8>(p, head_dim, s.rb, batch, stream);
   if (dtype == KVE_BF16) return launch_hd<kBf16>(p, head_dim, s.rb, batch, stream);
   return launch_hd<kF32>(p, head_dim, s.rb, batch, stream);
 }

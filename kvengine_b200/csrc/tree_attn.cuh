@@ -45,6 +45,12 @@ __device__ __forceinline__ int node_of(const TreeParams& p, int r) {
 size_t tree_attn_wide_partial_bytes(int batch, int max_q, int max_ctx, int nkv, int group, int hd);
 int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, cudaStream_t stream);
 
+// The kernel for at most eight rows (tree_attn_small.cu): whether it takes a call (bf16 queries), its
+// partials, and the call.
+bool tree_attn_small_takes(const TreeParams& p, bool fp8);
+size_t tree_attn_small_partial_bytes(int batch, int max_ctx, int nkv, int hd);
+int tree_attn_small(TreeParams p, int batch, int max_ctx, int hd, bool fp8, cudaStream_t stream);
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -792,7 +792,7 @@ WidePlan wide_plan(int batch, int max_q, int max_ctx, int nkv, int group) {
 bool pool_map(CUtensorMap* map, const void* pool, int64_t rows, int width, int hd, bool v) {
   EncodeTiledFn fn = encode_fn();
   if (!fn || width >= (1 << 24)) return false;
-  return cached_map(map, pool, (uint64_t)rows | (uint64_t)width << 32 | (uint64_t)(v ? hd : 0) << 56, [&](CUtensorMap* m) {
+  return cached_map(map, pool, (uint64_t)rows | (uint64_t)width << 32 | (uint64_t)(v ? hd / 64 : 0) << 56, [&](CUtensorMap* m) {
     cuuint64_t dims2[2] = {(cuuint64_t)width, (cuuint64_t)rows};
     cuuint64_t dims3[3] = {64, (cuuint64_t)rows, (cuuint64_t)width / 64};
     cuuint64_t strides[2] = {(cuuint64_t)width * 2, 128};

@@ -191,11 +191,45 @@ def test_tree_attention_same_rows_as_paged_attention_on_chains(cuda_device):
     assert bool(((a.double() - b.double()).abs().cpu() <= 2 * tol).all())
 
 
+@pytest.mark.parametrize("heads", [(2, 1, 128), (4, 4, 64), (8, 2, 64), (16, 2, 128)])
+@pytest.mark.parametrize("nodes, hists, bs, kind", [
+    ([1], [0], 16, "none"), ([1] * 5, [1, 15, 16, 31, 700], 16, "none"), ([2, 1, 2, 0, 1], [40, 0, 2100, 9, 32], 32, "tree"),
+    ([2, 2, 1], [14, 300, 95], 16, "random"), ([2, 1], [5000, 60], 48, "none")])
+@pytest.mark.parametrize("cache", ["bf16", "fp8"])
+def test_tree_attention_few_rows(cuda_device, cache, heads, nodes, hists, bs, kind):
+    """Single tokens and pairs: at most eight rows per kv head (sixteen in the last layout)."""
+    args, *lens = attention_case(cache, heads, nodes, hists, bs, kind, 23, cuda_device)
+    status = ops.status_tensor(cuda_device)
+    ws = ops.Workspace(cuda_device)
+    got = ops.tree_attention(**args, workspace=ws, status=status)
+    check_attention(args, *lens, got)
+    assert int(status) == 0 and int(ws.buf[:65536 if ws.buf.numel() > 65536 else 0].sum()) == 0
+    assert torch.equal(ops.tree_attention(**args, workspace=ws), got)
+
+
+def test_tree_attention_few_rows_bad_block(cuda_device):
+    """A block id outside the pool reads as zeros, its exponents too."""
+    for cache in ("bf16", "fp8"):
+        args, ctx, nodes, off = attention_case(cache, (8, 2, 64), [1, 1], [40, 70], 16, "none", 3, cuda_device)
+        want = ops.tree_attention(**args)
+        tables = args["block_tables"].clone()
+        tables[1, 1] = -1
+        status = ops.status_tensor(cuda_device)
+        got = ops.tree_attention(**dict(args, block_tables=tables), status=status)
+        assert int(status) == -7 and torch.equal(got[0], want[0]) and torch.isfinite(got.float()).all()
+        zero = dict(args)
+        for x in ("pool_k_layer", "pool_v_layer"):
+            zero[x] = args[x].clone()
+            zero[x].view(torch.uint8)[args["block_tables"][1, 1].long()] = 0
+        check_attention(zero, ctx, nodes, off, got)
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 64), (4, 4, 64), (2, 2, 128)])
 @pytest.mark.parametrize("cache", ["bf16", "fp32", "fp8"])
-def test_tree_attention_garbage_in_unseen_places(cuda_device, cache):
+def test_tree_attention_garbage_in_unseen_places(cuda_device, cache, heads):
     """Infinities and NaN in unused slots, in a partial page's tail and in nodes a row does not see
     reach no row that does not see them; a row that sees a NaN gets one."""
-    args, ctx, nodes, off = attention_case(cache, (4, 2, 64), [6, 4], [35, 3], 16, "tree", 21, cuda_device)
+    args, ctx, nodes, off = attention_case(cache, heads, [6, 4], [35, 3], 16, "tree", 21, cuda_device)
     clean = ops.tree_attention(**args)
     mask = ops.tree_mask_words([[-1, 0, 0, 1, 2, 2], [-1, -1, 0, 0]], 6)
     args["tree_mask"] = mask.to(cuda_device)
