@@ -140,6 +140,39 @@ def load() -> C.CDLL:
     return lib
 
 
+class _NoFast:
+    """Stands in for the C++ binding where it has not been built: it takes no call."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+_fast = None
+_FAST_CALLS = ("kve_paged_tree_attn", "kve_tree_attn_workspace_bytes", "kve_qkv_rope_append_fp8", "kve_kv_read_fp8",
+               "kve_sample_accept", "kve_sample_accept_workspace_bytes", "kve_tree_sample_accept",
+               "kve_tree_sample_accept_workspace_bytes", "kve_kv_commit_path")
+
+
+def fast():
+    """The C++ binding of a sampling step's ops (csrc/fastcall.cpp), bound to the library. A function
+    of it returns None for a call it does not take."""
+    global _fast
+    if _fast is None:
+        lib = load()
+        path = os.path.join(os.path.dirname(_LIB_PATH), "_fastcall.so")
+        if os.path.exists(path):
+            from importlib import machinery, util
+
+            loader = machinery.ExtensionFileLoader("kvengine_b200._fastcall", path)
+            module = util.module_from_spec(util.spec_from_loader("kvengine_b200._fastcall", loader))
+            loader.exec_module(module)
+            module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in _FAST_CALLS))
+            _fast = module
+        else:
+            _fast = _NoFast()
+    return _fast
+
+
 def check(rc: int) -> None:
     if rc != KVE_OK:
         msg = load().kve_last_error().decode(errors="replace")

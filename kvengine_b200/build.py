@@ -18,6 +18,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OBJDIR = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libkvengine_b200.so")
+FAST = os.path.join(PKG, "_fastcall.so")  # the C++ binding of a sampling step's ops (csrc/fastcall.cpp)
 SOURCES = ["capi.cu", "accept.cu", "kv.cu", "attention.cu", "gemm.cu", "gemm_simt.cu", "gemm_tc.cu",
            "forward.cu", "step.cu", "tree_attn.cu", "tree_attn_tc.cu", "tree_attn_small.cu",
            "kv_fp8.cu", "sample.cu", "kv_path.cu"]
@@ -66,7 +67,31 @@ def build(force: bool = False, verbose: bool = False) -> str:
         list(ex.map(run, jobs))
     if force or jobs or not _newer(LIB, objs):
         run([cc] + ARCH + ["-shared", "-o", LIB] + objs)
+    build_fastcall(force, verbose)
     return LIB
+
+
+def build_fastcall(force: bool = False, verbose: bool = False) -> str:
+    """The CPython extension that calls the library from C++ (host code only; torch's headers)."""
+    import sysconfig
+
+    import torch
+
+    src = os.path.join(CSRC, "fastcall.cpp")
+    if not force and _newer(FAST, [src, os.path.join(INCLUDE, "kvengine_b200.h")]):
+        return FAST
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home}/include",
+           f"-I{home}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", src,
+           "-o", FAST, f"-L{home}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"c++ failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    return FAST
 
 
 if __name__ == "__main__":

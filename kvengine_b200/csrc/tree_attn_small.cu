@@ -14,8 +14,8 @@
 //
 // A CTA takes one (sequence x kv head) and a chunk of the keys; each of its four warps is
 // a stream of its own: every fourth tile of the chunk, through a ring of its own that
-// its issuing lane fills by TMA (boxes of 16 keys; the exponents by bulk copies of a
-// block's 16 rows), with no barrier between warps before the end.
+// its issuing lane fills by TMA (boxes of 16 keys; the exponents by a 4-byte cp.async a
+// lane), with no barrier between warps before the end.
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -32,7 +32,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;
-constexpr int kMaxScale = 512;  // bytes of 16 keys' exponents (kv heads up to 32)
 
 template <bool FP8, int HD>
 struct SmallShape {
@@ -41,13 +40,13 @@ struct SmallShape {
   static constexpr int GROUPS = GROUP >= 4096 ? 1 : 2;      // of a tile
   static constexpr int KEYS = 16 * GROUPS;
   static constexpr int PAIR = 2 * GROUPS * GROUP;           // K and V of a tile
-  static constexpr int NST = 24576 / PAIR < 6 ? 24576 / PAIR : 6;  // tiles of a warp's ring
+  static constexpr int NST = 16384 / PAIR;                  // tiles of a warp's ring
   static constexpr int RINGS = kWarps * NST * PAIR;
   static constexpr int XROW = HD + 4;
   static constexpr int MERGE = kWarps * kRows * (XROW + 2) * 4;
   static constexpr int AREA = RINGS > MERGE ? RINGS : MERGE;
   static constexpr int ROWB = HD * ELEM < 128 ? 64 : 128;   // bytes of a box row
-  static size_t smem(int nkv) { return 1024 + AREA + (FP8 ? (size_t)kWarps * NST * 2 * GROUPS * 16 * nkv : 0); }
+  static constexpr size_t SMEM = 1024 + AREA + (FP8 ? kWarps * NST * 256 : 0);  // a word per key for K's and V's exponents
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -120,16 +119,8 @@ __device__ __forceinline__ void tma_box(uint32_t lead, uint32_t dst, const CUten
       "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void bulk_copy(uint32_t lead, uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\t"
-      "setp.ne.b32 q, %4, 0;\n\t"
-      "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
-      ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "r"(lead) : "memory");
-}
-
 template <bool FP8, int HD>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
 tree_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeParams p) {
   using S = SmallShape<FP8, HD>;
   constexpr int NST = S::NST, GROUPS = S::GROUPS, KEYS = S::KEYS;
@@ -141,7 +132,7 @@ tree_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int g = lane >> 2, tq = lane & 3;
   if (threadIdx.x == 0) {
     for (int w = 0; w < kWarps; ++w)
-      for (int i = 0; i < NST; ++i) mbar_init(smem_u32(&full[w][i]), 1);
+      for (int i = 0; i < NST; ++i) mbar_init(smem_u32(&full[w][i]), FP8 ? 33 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&map_k);
     prefetch_map(&map_v);
@@ -167,10 +158,10 @@ tree_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
   __syncthreads();
 
-  // The ring: [stage][K groups, V groups], and for e4m3 [stage][K, V][group][16 keys][kv heads] exponents.
+  // The ring: [stage][K groups, V groups], and for e4m3 [stage][K, V][key]: the aligned word that holds
+  // the key's exponent byte.
   const uint32_t ring = smem_u32(smem) + warp * NST * S::PAIR;
-  const int sbytes = 16 * p.nkv;
-  const uint32_t sring = smem_u32(smem) + S::AREA + warp * NST * 2 * GROUPS * sbytes;
+  const uint32_t sring = smem_u32(smem) + S::AREA + warp * NST * 256;
   const uint32_t lead = elect_lane();
   // Lane l knows where group l of a window of 32 groups (16 keys each) of this warp's tiles lies.
   const int past = (int)(p.num_blocks * p.bs);
@@ -194,32 +185,26 @@ tree_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
     const int st = i % NST;
     const uint32_t bar = smem_u32(&full[warp][st]), dst = ring + st * S::PAIR;
-    int y[GROUPS];
-    uint32_t bytes = S::PAIR;
-#pragma unroll
-    for (int u = 0; u < GROUPS; ++u) {
-      y[u] = __shfl_sync(0xffffffffu, now, i % WINDOW * GROUPS + u);
-      if (FP8 && y[u] < past) bytes += 2 * sbytes;
-    }
-    if (lead) mbar_expect_tx(bar, bytes);
+    if (lead) mbar_expect_tx(bar, S::PAIR);
     __syncwarp();
 #pragma unroll
     for (int u = 0; u < GROUPS; ++u) {
+      const int y = __shfl_sync(0xffffffffu, now, i % WINDOW * GROUPS + u);
 #pragma unroll
       for (int half = 0; half < (HD * S::ELEM + 127) / 128; ++half) {
-        const uint32_t at = dst + u * S::GROUP + half * 2048;
-        tma_box(lead, at, &map_k, h * HD + half * 64, y[u], bar);
-        tma_box(lead, at + GROUPS * S::GROUP, &map_v, h * HD + half * 64, y[u], bar);
+        const uint32_t to = dst + u * S::GROUP + half * 2048;
+        tma_box(lead, to, &map_k, h * HD + half * 64, y, bar);
+        tma_box(lead, to + GROUPS * S::GROUP, &map_v, h * HD + half * 64, y, bar);
       }
-      if (FP8 && y[u] < past) {
-        const uint32_t at = sring + (st * 2 * GROUPS + u) * sbytes;
-        bulk_copy(lead, at, p.k_scale + (size_t)y[u] * p.nkv, sbytes, bar);
-        bulk_copy(lead, at + GROUPS * sbytes, p.v_scale + (size_t)y[u] * p.nkv, sbytes, bar);
-      } else if (FP8 && lane * 16 < sbytes) {
-        const uint32_t at = sring + (st * 2 * GROUPS + u) * sbytes + lane * 16;
-        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0u) : "memory");
-        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at + GROUPS * sbytes), "r"(0u) : "memory");
-      }
+    }
+    if constexpr (FP8) {
+      // lane l: key l of the tile
+      const int y = __shfl_sync(0xffffffffu, now, i % WINDOW * GROUPS + lane / 16);
+      const size_t word = y < past ? (((size_t)(y + lane % 16) * p.nkv + h) & ~(size_t)3) : 0;
+      const uint32_t to = sring + st * 256 + lane * 4, bytes = y < past ? 4u : 0u;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(p.k_scale + word), "r"(bytes) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 128), "l"(p.v_scale + word), "r"(bytes) : "memory");
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     }
   };
   for (int i = 0; i < NST && i < my_tiles; ++i) load(i);
@@ -297,7 +282,7 @@ tree_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
     const int kt = key_lo + (warp + kWarps * i) * KEYS;
     const uint32_t kb = ring + st * S::PAIR, vb = kb + GROUPS * S::GROUP;
-    const uint32_t ks = sring + st * 2 * GROUPS * sbytes + h;
+    const uint32_t ks = sring + st * 256 + ((g * p.nkv + h) & 3);  // + 4 key: the byte of keys g and g + 8
     const bool masked = kt + KEYS > hist || kt + KEYS > key_hi;
     bool odd = false;
     if (masked) {
@@ -362,10 +347,10 @@ tree_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           for (int w = 0; w < 4; ++w)
             mma<true>(s[u], to_f16(x[dg][0][w] & 0xffffu), to_f16(x[dg][1][w] & 0xffffu), to_f16(x[dg][0][w] >> 16),
                       to_f16(x[dg][1][w] >> 16), qb[dg * 4 + w][0], qb[dg * 4 + w][1]);
-        const float k0 = scale_value(lds8(ks + u * sbytes + g * p.nkv));
-        const float k1 = scale_value(lds8(ks + u * sbytes + (g + 8) * p.nkv));
-        vs[u][0] = scale_value(lds8(ks + (GROUPS + u) * sbytes + g * p.nkv));
-        vs[u][1] = scale_value(lds8(ks + (GROUPS + u) * sbytes + (g + 8) * p.nkv));
+        const float k0 = scale_value(lds8(ks + (u * 16 + g) * 4));
+        const float k1 = scale_value(lds8(ks + (u * 16 + g + 8) * 4));
+        vs[u][0] = scale_value(lds8(ks + 128 + (u * 16 + g) * 4));
+        vs[u][1] = scale_value(lds8(ks + 128 + (u * 16 + g + 8) * 4));
         s[u][0] *= k0;
         s[u][1] *= k0;
         s[u][2] *= k1;
@@ -604,9 +589,11 @@ tree_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 }
 
 // ------------------------------------------------------------------ host
-// Chunks of a sequence: enough CTAs for about four waves of two an SM, none under 256 keys.
+// Chunks of a sequence, none under 256 keys: full-length sequences would make a third more than the 444
+// CTAs that run at once, a ragged batch about as many (64 requests of 2250 to 9000 keys: 50 us; with
+// twice the chunks 56, with fewer 59).
 void small_split(int batch, int max_ctx, int nkv, int* chunk, int* n_chunks) {
-  const long long units = (long long)batch * nkv, want = 4 * 2 * 148;
+  const long long units = (long long)batch * nkv, want = 4 * 148;
   const long long c = (want + units - 1) / units;
   long long keys = ((long long)max_ctx + c - 1) / c;
   keys = (keys + 127) / 128 * 128;
@@ -647,14 +634,14 @@ int launch(const TreeParams& p, int batch, cudaStream_t stream) {
   const uint64_t bit = 1ull << (dev & 63);
   if (err == cudaSuccess && !(prepared.load(std::memory_order_relaxed) & bit)) {
     err = cudaFuncSetAttribute(tree_attn_small_kernel<FP8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)S::smem(kMaxScale / 16));
+                               (int)S::SMEM);
     if (err == cudaSuccess) prepared.fetch_or(bit, std::memory_order_relaxed);
   }
   if (err != cudaSuccess) {
     cudaGetLastError();
     return set_error(KVE_ERR_CUDA, "kve_paged_tree_attn: %s", cudaGetErrorString(err));
   }
-  launch_kernel(tree_attn_small_kernel<FP8, HD>, dim3(batch * p.nkv, p.n_chunks), dim3(kThreads), S::smem(FP8 ? p.nkv : 0),
+  launch_kernel(tree_attn_small_kernel<FP8, HD>, dim3(batch * p.nkv, p.n_chunks), dim3(kThreads), S::SMEM,
                 stream, mk, mv, p);
   return check_launch("kve_paged_tree_attn(small)");
 }
@@ -663,7 +650,7 @@ int launch(const TreeParams& p, int batch, cudaStream_t stream) {
 
 bool tree_attn_small_takes(const TreeParams& p, bool fp8) {
   if ((long long)p.max_q * p.group > kRows || p.bs % 16 || p.num_blocks * p.bs >= 0x7ffffff0LL) return false;
-  return !fp8 || (p.nkv * 16 <= kMaxScale && (uintptr_t)p.k_scale % 16 == 0 && (uintptr_t)p.v_scale % 16 == 0);
+  return !fp8 || ((uintptr_t)p.k_scale % 4 == 0 && (uintptr_t)p.v_scale % 4 == 0);
 }
 
 size_t tree_attn_small_partial_bytes(int batch, int max_ctx, int nkv, int hd) {

@@ -238,8 +238,9 @@ def spec_next_draft_plan(start_lens: torch.Tensor, last_tokens: torch.Tensor, n_
 
 
 # ------------------------------------------------ sampling, draft trees and the 8-bit cache
-# These calls are a few microseconds of GPU work in a decode step, so their checks are
-# kept to a few attribute reads per tensor and the message is made only for a failure.
+# These calls are a few microseconds of GPU work in a decode step: the C++ binding takes them
+# where everything is as it should be, and what it leaves (it returns None) is checked and
+# called here, where the errors are raised.
 _I32, _F32, _U8, _E4M3 = torch.int32, torch.float32, torch.uint8, torch.float8_e4m3fn
 
 
@@ -304,6 +305,13 @@ def tree_attention(q, pool_k_layer, pool_v_layer, block_tables, ctx_lens, q_lens
     whether it sees node t of its sequence (`tree_mask_words` builds it from parents; None: a
     chain); a row that sees nothing gets zeros. bf16 queries also read an e4m3 cache, given
     its layer's k_scale and v_scale [num_blocks, bs, nkv] uint8."""
+    r = L.fast().tree_attention(q, pool_k_layer, pool_v_layer, block_tables, ctx_lens, q_lens, q_offsets, max_q_len,
+                                max_ctx, scale, tree_mask, k_scale, v_scale, out,
+                                None if workspace is None else workspace.buf, status)
+    if r is not None:
+        if r.__class__ is int:
+            L.check(r)
+        return r
     lib = L.load()
     dev = _device(q)
     n, nq, hd = q.shape
@@ -373,6 +381,12 @@ def qkv_rope_append_fp8(qkv, positions, slots, rope_cos, rope_sin, q_out, pool_k
                         num_heads, num_kv_heads, head_dim, status=None) -> None:
     """`qkv_rope_append` into an e4m3 cache (pools [num_blocks, bs, nkv, hd] float8_e4m3fn, scales
     [num_blocks, bs, nkv] uint8): q rotated into q_out, K rotated and quantised, V quantised."""
+    r = L.fast().qkv_rope_append_fp8(qkv, positions, slots, rope_cos, rope_sin, q_out, pool_k_layer, pool_v_layer,
+                                     k_scale, v_scale, num_heads, num_kv_heads, head_dim, status)
+    if r is not None:
+        if r.__class__ is int:
+            L.check(r)
+        return
     lib = L.load()
     name = "qkv_rope_append_fp8"
     dev, dtype = _device(qkv), qkv.dtype
@@ -413,6 +427,12 @@ def kv_read_fp8(pool_k_layer, pool_v_layer, k_scale, v_scale, slot_ids, dtype: t
                 status=None):
     """Rows of an e4m3 cache as the values they stand for: (k, v), each [n, nkv, hd] in `dtype`, of
     the flat slots slot_ids [n] int64. `out` may give the two."""
+    if out is None and (dtype is torch.bfloat16 or dtype is _F32):
+        r = L.fast().kv_read_fp8(pool_k_layer, pool_v_layer, k_scale, v_scale, slot_ids, int(dtype is torch.bfloat16), status)
+        if r is not None:
+            if r.__class__ is int:
+                L.check(r)
+            return r
     lib = L.load()
     dev = _device(pool_k_layer)
     num_blocks, bs, nkv, hd = pool_k_layer.shape
@@ -451,6 +471,13 @@ def sample_accept(logits: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Te
     strides), uniforms [B, k] in [0, 1), gumbel [B, V] noise -log(-log u), temperature [B]
     (0: greedy), draft_logits [B, k, V] (None: drafts without a distribution) ->
     (n_accepted [B], emitted [B, k+1], logprobs [B, k+1]). `out` may give the three."""
+    if out is None:
+        r = L.fast().sample_accept(logits, drafts, uniforms, gumbel, temperature, draft_logits,
+                                   None if workspace is None else workspace.buf, status)
+        if r is not None:
+            if r.__class__ is int:
+                L.check(r)
+            return r
     lib = L.load()
     name = "sample_accept"
     dev, dtype = _device(logits), logits.dtype
@@ -501,6 +528,13 @@ def tree_sample_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torc
     parents (int32), uniforms [N] of the trees' nodes, sequence b's at rows q_offsets[b] .. +
     q_lens[b] (parents within the tree, node 0 its root); gumbel [B, V], temperature [B] ->
     (n_accepted [B], path, emitted, logprobs [B, max_q_len]). `out` may give the four."""
+    if out is None:
+        r = L.fast().tree_sample_accept(logits, tokens, parents, q_lens, q_offsets, max_q_len, uniforms, gumbel,
+                                        temperature, None if workspace is None else workspace.buf, status)
+        if r is not None:
+            if r.__class__ is int:
+                L.check(r)
+            return r
     lib = L.load()
     name = "tree_sample_accept"
     dev, dtype = _device(logits), logits.dtype
@@ -539,6 +573,11 @@ def kv_commit_path(pool_k, pool_v, block_tables, start_lens, path, n_accepted, k
     n_accepted[b], position start_lens[b] + path[b, j] -> start_lens[b] + j. pools [L, num_blocks, bs,
     nkv, hd] (an e4m3 cache with its scales [L, num_blocks, bs, nkv]); path [B, P] and n_accepted
     [B] int32 as `tree_sample_accept` gives them; start_lens [B] the positions of the trees' node 0."""
+    r = L.fast().kv_commit_path(pool_k, pool_v, block_tables, start_lens, path, n_accepted, k_scale, v_scale, status)
+    if r is not None:
+        if r.__class__ is int:
+            L.check(r)
+        return
     lib = L.load()
     dev = _device(pool_k)
     layers, num_blocks, bs, nkv, hd = pool_k.shape
