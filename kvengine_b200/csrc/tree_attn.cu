@@ -711,29 +711,28 @@ tree_attn_kernel(TreeParams p) {
 }
 
 // ------------------------------------------------------------------ host
-// Row blocks of 16 query rows in a CTA, from the rows of the call's largest tree.
-int row_blocks(int max_q, int group) {
-  const long long rows = (long long)max_q * group;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-}
-
 struct Split {
   int rb, n_qtiles, chunk, n_chunks;
 };
 
-// Chunks: as many CTAs as fill the SMs about four times over, no chunk under 128
-// keys (below that its fixed costs outweigh its keys). Only grids of fewer tiles
-// than that are split, so the counters always suffice.
+// Row blocks of 16 query rows in a CTA from the rows of the call's largest tree, fewer where the
+// grid would leave SMs idle (each key then passes through more CTAs, from L2, and more streams of keys
+// run side by side). Chunks: as many CTAs as fill the SMs about four times over, none under 128 keys
+// (64 in a grid of under one CTA an SM), below which a chunk's fixed costs outweigh its keys. Only
+// grids of fewer tiles than that are split, so the counters always suffice.
 Split split_of(int batch, int max_q, int max_ctx, int nkv, int group) {
+  const long long rows = (long long)max_q * group, seqs = (long long)batch * nkv;
   Split s;
-  s.rb = row_blocks(max_q, group);
-  s.n_qtiles = (int)(((long long)max_q * group + s.rb * 16 - 1) / (s.rb * 16));
-  const long long units = (long long)batch * nkv * s.n_qtiles;
-  const long long want = 4 * 2 * 148;
-  long long chunks = (want + units - 1) / units;
+  s.rb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  auto tiles = [&](int rb) { return seqs * ((rows + rb * 16 - 1) / (rb * 16)); };
+  while (s.rb > 1 && tiles(s.rb) * ((max_ctx + 127) / 128) < 148) s.rb /= 2;
+  const long long units = tiles(s.rb);
+  s.n_qtiles = (int)((rows + s.rb * 16 - 1) / (s.rb * 16));
+  const long long least = units * ((max_ctx + 127) / 128) < 148 ? 64 : 128;
+  const long long chunks = (4 * 2 * 148 + units - 1) / units;
   long long chunk = ((long long)max_ctx + chunks - 1) / chunks;
   chunk = (chunk + 63) / 64 * 64;
-  chunk = chunk < 128 ? 128 : chunk;
+  chunk = chunk < least ? least : chunk;
   s.chunk = (int)chunk;
   s.n_chunks = (int)((max_ctx + chunk - 1) / chunk);
   if (s.n_chunks < 1) s.n_chunks = 1;
@@ -744,9 +743,10 @@ size_t partial_bytes(const Split& s, int batch, int nkv, int hd) {
   return (size_t)batch * nkv * s.n_qtiles * s.n_chunks * (s.rb * 16) * (hd + 4) * sizeof(float);
 }
 
-// The wide kernel's tile is 128 rows: it is for trees of more rows than this per kv head.
-constexpr int kWideRows = 32;
-bool use_wide(int max_q, int group) { return (long long)max_q * group > kWideRows; }
+// More than the few-row kernel's eight rows go to the wide kernel, although its tile is 128 rows: 24 rows
+// (64 sequences of up to 700 keys) took it 13.2 us against 25.8 here, 16 rows (16 sequences, 8 kv heads,
+// 3000 keys) 32.9 against 42.2, one sequence of 32 rows 9.4 against 10.1.
+bool use_wide(int max_q, int group) { return (long long)max_q * group > 8; }
 
 template <int KV, int HD, int RB>
 int launch(const TreeParams& p, int batch, cudaStream_t stream) {
