@@ -8,15 +8,19 @@
 // those whose bit is set in the row's mask words (without a mask: itself and the
 // ones before it). A row that sees nothing gets zeros.
 //
+// Three kernels, by what bounds them:
+//   tree_attn_small.cu  up to 8 rows (nodes x heads of a kv head): the cache's bytes
+//   tree_attn_tc.cu     more: the tensor cores (tcgen05)
+//   this file           fp32, and what those two cannot load by TMA (bf16 and few-row e4m3 caches with
+//                       blocks that are no multiple of 16)
+//
 // The work is one pass over the keys with a running maximum and sum. A CTA takes
 // one (sequence x kv head), a tile of up to 64 query rows (row = node x group
 // head) and a chunk of the keys; its four warps are RB row blocks of 16 rows
 // times KS = 4 / RB key streams. Key tile t (16 keys) of the chunk belongs to
 // stream t mod KS, and each stream has its own ring of tiles in shared memory
 // that its warps fill with 16-byte cp.async, so any block size and any head
-// stride works, no warp waits for another stream, and about 100 KB a CTA (two
-// CTAs an SM) are in flight against the latency of HBM. Few rows make the cache's
-// bytes the bound: each K/V byte is then read once per call.
+// stride works and no warp waits for another stream.
 //
 // The products run on the tensor cores:
 //   bf16  m16n8k16 on bf16. P is rounded to bf16 for P V (its sum is not).
@@ -69,10 +73,6 @@ __device__ __forceinline__ uint32_t e4m3_to_bf16x2(uint32_t two) {
   __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
   const float2 f = __half22float2(__half2(h));
   return bf16x2(f.x, f.y);
-}
-// 2^(byte - 127); byte 255 stands for NaN.
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-  return byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -770,9 +770,12 @@ int launch(const TreeParams& p, int batch, cudaStream_t stream) {
 }
 template <int KV, int HD>
 int launch_rb(const TreeParams& p, int rb, int batch, cudaStream_t stream) {
-  if (rb == 1) return launch<KV, HD, 1>(p, batch, stream);
-  if (rb == 2) return launch<KV, HD, 2>(p, batch, stream);
-  return launch<KV, HD, 4>(p, batch, stream);
+  // e4m3 comes here with at most eight rows (and blocks that the few-row kernel does not take)
+  if (KV == kFp8 || rb == 1) return launch<KV, HD, 1>(p, batch, stream);
+  if constexpr (KV != kFp8) {
+    if (rb == 2) return launch<KV, HD, 2>(p, batch, stream);
+    return launch<KV, HD, 4>(p, batch, stream);
+  }
 }
 template <int KV>
 int launch_hd(const TreeParams& p, int hd, int rb, int batch, cudaStream_t stream) {
@@ -839,8 +842,8 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
   const bool fp8 = kv_dtype == KVE_FP8_E4M3;
   const Split s = split_of(batch, max_q_len, max_ctx, num_kv_heads, group);
   const bool small = dtype == KVE_BF16 && tree_attn_small_takes(p, fp8);
-  const bool wide = !small && kv_dtype == KVE_BF16 && use_wide(max_q_len, group) && block_size % 16 == 0 &&
-                    num_blocks * block_size < 0x7ffffff0LL;
+  const bool wide = !small && use_wide(max_q_len, group) &&
+                    (fp8 || (dtype == KVE_BF16 && block_size % 16 == 0 && num_blocks * block_size < 0x7ffffff0LL));
   const size_t part = small  ? tree_attn_small_partial_bytes(batch, max_ctx, num_kv_heads, head_dim)
                       : wide ? tree_attn_wide_partial_bytes(batch, max_q_len, max_ctx, num_kv_heads, group, head_dim)
                              : partial_bytes(s, batch, num_kv_heads, head_dim);
@@ -851,7 +854,7 @@ extern "C" int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k,
   p.partials = part ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kTreeCounterBytes) : nullptr;
   p.chunk = s.chunk; p.n_chunks = s.n_chunks; p.n_qtiles = s.n_qtiles;
   if (small) return tree_attn_small(p, batch, max_ctx, head_dim, fp8, stream);
-  if (wide) return tree_attn_wide(p, batch, max_ctx, head_dim, stream);
+  if (wide) return tree_attn_wide(p, batch, max_ctx, head_dim, fp8, stream);
   if (fp8) return launch_hd<kFp8>(p, head_dim, s.rb, batch, stream);
   if (dtype == KVE_BF16) return launch_hd<kBf16>(p, head_dim, s.rb, batch, stream);
   return launch_hd<kF32>(p, head_dim, s.rb, batch, stream);

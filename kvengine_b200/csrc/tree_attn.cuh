@@ -40,16 +40,20 @@ __device__ __forceinline__ int node_of(const TreeParams& p, int r) {
   return p.group == 1 ? r : (int)__umulhi((uint32_t)r, p.group_inv);
 }
 
-// The wide kernel (tree_attn_tc.cu): its partials of a call, and the call itself. bf16, a
-// block size of a multiple of 16, a pool of under 2^31 - 16 rows.
+// The wide kernel (tree_attn_tc.cu): its partials of a call, and the call itself: e4m3
+// caches, and bf16 ones with a block size of a multiple of 16 and a pool of under 2^31 - 16 rows.
 size_t tree_attn_wide_partial_bytes(int batch, int max_q, int max_ctx, int nkv, int group, int hd);
-int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, cudaStream_t stream);
+int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, bool fp8, cudaStream_t stream);
 
 // The kernel for at most eight rows (tree_attn_small.cu): whether it takes a call (bf16 queries), its
 // partials, and the call.
 bool tree_attn_small_takes(const TreeParams& p, bool fp8);
 size_t tree_attn_small_partial_bytes(int batch, int max_ctx, int nkv, int hd);
 int tree_attn_small(TreeParams p, int batch, int max_ctx, int hd, bool fp8, cudaStream_t stream);
+// 2^(byte - 127); byte 255 stands for NaN.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

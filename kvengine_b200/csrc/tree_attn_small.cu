@@ -66,9 +66,6 @@ __device__ __forceinline__ uint32_t to_bf16(uint32_t two) {
   const float2 f = __half22float2(__half2(h));
   return pack2(f.x, f.y);
 }
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-  return byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
-}
 template <bool F16>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (F16)

@@ -1,8 +1,9 @@
 // Tree attention for many query rows per kv head, on the 5th-generation tensor cores.
 //
-// The same operation as tree_attn.cu for bf16 caches, where a sequence's tree has more
-// rows (nodes x group heads) than the tile of m16 products can hide: the work is then
-// bound by the tensor cores and the exponentials rather than by the cache's bytes.
+// The same operation as tree_attn.cu for bf16 and e4m3 caches, where a sequence's tree has
+// more rows (nodes x group heads) than the few-row kernel takes: the work is then bound by
+// the tensor cores and the exponentials rather than by the cache's bytes. e4m3 tiles become
+// bf16 on their way into shared memory (exactly: e4m3 times a power of two).
 //
 // A CTA has two softmax warpgroups, each with two 128-row score tiles S and one output
 // tile O in tensor memory, and one of two jobs:
@@ -27,6 +28,7 @@
 // zeroed (the pool's contents there are not this sequence's), and new tokens' rows are
 // checked for infinities and NaN, which 0 x V would spread to rows that do not see them.
 // Where there are any, the chunk's rows are computed again, key by key.
+#include <cuda_fp8.h>
 #include <math.h>
 
 #include <atomic>
@@ -43,6 +45,7 @@ namespace {
 constexpr int kKeys = 64;        // keys of a tile
 constexpr int kRows = 128;       // query rows of a tile
 constexpr int kThreads = 384;    // loader, a warp of products for each group, V warp; two softmax warpgroups
+constexpr int threads_of(bool fp8) { return kThreads + (fp8 ? 128 : 0); }  // e4m3: four warps that copy
 constexpr int kMaxSlots = 12;
 constexpr int kShare = 4;        // every kShare-th pair of exponentials runs on the fp32 units
 
@@ -212,8 +215,8 @@ struct WideShape {
   static_assert(SMEM <= 232448, "shared memory");
 };
 
-template <int HD, bool TWO>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int HD, bool TWO, bool FP8>
+__global__ void __launch_bounds__(threads_of(FP8), 1)
 tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeParams p) {
   using W = WideShape<HD, TWO>;
   constexpr int NS = W::NS;
@@ -263,8 +266,8 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(smem_u32(&full[i]), 1);
-      mbar_init(smem_u32(&ready[i]), 1);
+      mbar_init(smem_u32(&full[i]), FP8 ? 2 : 1);  // e4m3: the two warps that copy its tiles
+      mbar_init(smem_u32(&ready[i]), FP8 ? 2 : 1);
       mbar_init(smem_u32(&empty[i]), TWO && steps1 > 0 ? 2 : 1);  // one commit of each group that reads it
     }
     for (int g = 0; g < 2; ++g) {
@@ -277,8 +280,10 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     *odd = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    prefetch_map(&map_k);
-    prefetch_map(&map_v);
+    if constexpr (!FP8) {
+      prefetch_map(&map_k);
+      prefetch_map(&map_v);
+    }
   }
   __syncthreads();  // the barriers are there: the copies may start
   // K tile t lies in slot t mod NK, V tile t in slot NK + t mod NK; each slot has its barriers.
@@ -297,7 +302,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int gr = row0 + r, node = node_of(p, gr);
     return ((size_t)(qoff + node) * p.nq + h * p.group + gr - node * p.group) * HD;
   };
-  if (warp >= 4) {
+  if (warp >= 4 && warp < 12) {
     // Q into shared memory, 16 bytes a lane; a negative scale is a sign on q.
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
     // TWO: each group its own tile; else half of the one
@@ -321,7 +326,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     fence_proxy_async_smem();
   }
   uint32_t tmem = 0;
-  if (warp != 0) {  // Q and tensor memory are there
+  if (warp != 0 && warp < 12) {  // Q and tensor memory are there
     tc_before();
     asm volatile("bar.sync 2, 352;" ::: "memory");
     tc_after();
@@ -344,7 +349,125 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     return y;
   };
-  if (warp == 0) {
+  // e4m3: two warps copy K and two V, 32 of a tile's keys each, through their registers into the places
+  // where TMA puts bf16 tiles, as the bf16 numbers they stand for. The bytes are asked for two tiles
+  // ahead. (One warp for all of K or V, one tile ahead, took 8000 cycles a tile.)
+  auto copy_fp8 = [&](bool v, int half) {
+    constexpr int PIECES = HD / 16, PER = PIECES;  // 16-byte pieces of a key; a lane's, of a tile
+    constexpr int AT_ONCE = 32 / PIECES;           // keys of one load
+    const uint8_t* pool = static_cast<const uint8_t*>(v ? p.pool_v : p.pool_k) + (size_t)h * HD + lane % PIECES * 16;
+    const uint8_t* scales = (v ? p.v_scale : p.k_scale) + h;
+    const int32_t* table = p.tables + (size_t)b * p.table_stride;
+    uint4 bytes[2][PER];
+    uint32_t valid[2], byte[2];  // bit u: piece u's key is there; the exponent of this lane's key
+    auto key_of = [&](int t) { return key_lo + t * kKeys + 32 * half + lane; };
+    auto id_of = [&](int t) { return t < n && key_of(t) < key_hi ? table[key_of(t) / p.bs] : -1; };
+    auto ask = [&](int t, int id, int at) {  // tile t's bytes and exponents, `id` its block
+      const int key = key_of(t);
+      int slot = -1;
+      uint32_t e = 0;
+      if (key < key_hi) {
+        if (id >= 0 && id < p.num_blocks) {
+          slot = id * p.bs + key % p.bs;
+          e = scales[(size_t)slot * p.nkv];
+        } else if (!v) {
+          report(p.status, KVE_ERR_BOUNDS);  // reads as zeros
+        }
+      }
+      byte[at] = e;
+      valid[at] = 0;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const int sl = __shfl_sync(0xffffffffu, slot, u * AT_ONCE + lane / PIECES);
+        valid[at] |= (sl >= 0 ? 1u : 0u) << u;
+        bytes[at][u] = *reinterpret_cast<const uint4*>(pool + (size_t)(uint32_t)max(sl, 0) * (uint32_t)(p.nkv * HD));
+      }
+    };
+    auto store = [&](uint8_t* to, int u, const uint32_t (&o)[8]) {
+      const int r = 32 * half + u * AT_ONCE + lane / PIECES;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int piece = lane % PIECES * 2 + j;  // of the row's 8-element pieces
+        const size_t at = v ? (size_t)(r / 16) * (16 * HD * 2) + piece / 8 * 2048 + r % 16 * 128
+                            : (size_t)(piece / 8) * (kKeys * 128) + r * 128;
+        *reinterpret_cast<uint4*>(to + at + ((piece % 8 ^ (r & 7)) << 4)) =
+            make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+      }
+    };
+    bool found = false;
+    int id = id_of(2);
+    ask(0, id_of(0), 0);
+    if (n > 1) ask(1, id_of(1), 1);
+    auto tile = [&](int t, int at) {  // `at`: t mod 2, known when compiled
+      uint4 now[PER];
+      // A byte's exponent and mantissa, put where bf16 has the low bits of its exponent and
+      // the top of its mantissa, are the number times 2^-120, subnormals included: one product
+      // with 2^(e - 127 + 120) makes it the bf16 that it stands for. Not where that power
+      // is no bf16, nor for NaN bytes: such a tile goes through the conversions.
+      uint32_t odd_bytes = 0;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const uint32_t keep = valid[at] >> u & 1 ? ~0u : 0u;
+        now[u] = make_uint4(bytes[at][u].x & keep, bytes[at][u].y & keep, bytes[at][u].z & keep, bytes[at][u].w & keep);
+        odd_bytes |= ((now[u].x & 0x7f7f7f7fu) + 0x01010101u) | ((now[u].y & 0x7f7f7f7fu) + 0x01010101u) |
+                     ((now[u].z & 0x7f7f7f7fu) + 0x01010101u) | ((now[u].w & 0x7f7f7f7fu) + 0x01010101u);
+      }
+      const uint32_t e = byte[at];
+      if (t + 2 < n) {
+        ask(t + 2, id, at);
+        id = id_of(t + 3);
+      }
+      if (t >= NK) ok = ok && mbar_wait(smem_u32(&empty[slot_of(v, t)]), parity_of(t - NK), p.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      uint8_t* to = ring + (size_t)slot_of(v, t) * W::SLOT;
+      const bool plain = !__any_sync(0xffffffffu, (odd_bytes & 0x80808080u) != 0 || e > 134);
+      const uint32_t mine = plain ? ((e + 120) << 7) * 0x10001u : __float_as_uint(scale_value(e));
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const uint32_t up = __shfl_sync(0xffffffffu, mine, u * AT_ONCE + lane / PIECES);
+        const uint32_t w[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
+        uint32_t o[8];
+        if (plain) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t x = __byte_perm(w[i / 2], 0, i % 2 ? 0x3424 : 0x1404);
+            const uint32_t y = (x & 0x80008000u) | (x >> 4 & 0x07f007f0u);
+            const __nv_bfloat162 z = __hmul2(reinterpret_cast<const __nv_bfloat162&>(y), reinterpret_cast<const __nv_bfloat162&>(up));
+            o[i] = reinterpret_cast<const uint32_t&>(z);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (i % 2 * 16)), __NV_E4M3);
+            const float2 f = __half22float2(__half2(two));
+            o[i] = pack2(f.x * __uint_as_float(up), f.y * __uint_as_float(up));
+          }
+        }
+        store(to, u, o);
+        if (v && t >= special) {  // infinities and NaN in new tokens' rows
+          const int key = key_lo + t * kKeys + 32 * half + u * AT_ONCE + lane / PIECES;
+          if (key >= hist && key < key_hi) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) found |= odd_bits(o[i]);
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      if (__any_sync(0xffffffffu, found) && lane == 0) *odd = 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(v && t >= special ? &ready[(t - special) % NK] : &full[slot_of(v, t)]));
+    };
+    for (int t = 0; t < n && ok; t += 2) {
+      tile(t, 0);
+      if (t + 1 < n && ok) tile(t + 1, 1);
+    }
+  };
+  if (FP8 && (warp == 0 || warp >= 12)) {
+    if constexpr (FP8) {
+      if (warp >= 12) copy_fp8(warp & 1, (warp >> 1) & 1);
+    }
+  } else if (warp == 0) {
     // ---- K: boxes of 16 keys x 64 dims
     const uint32_t lead = elect_lane();
     int now = rows_of(0, true), next = rows_of(1, true);
@@ -444,7 +567,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     };
     const uint32_t lead = elect_lane();
     int now = rows_of(0, false), next = rows_of(1, false), looked = special;
-    for (int t = 0; t < n; ++t) {
+    for (int t = 0; t < n && !FP8; ++t) {
       if (t > 0 && t % 8 == 0) {
         now = next;
         next = rows_of(t / 8 + 1, false);
@@ -467,7 +590,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       if (looked < t && __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&full[slot_of(true, looked)]), parity_of(looked))))
         look(looked++);
     }
-    while (ok && looked < n) look(looked++);
+    while (!FP8 && ok && looked < n) look(looked++);
   } else if (warp >= 4) {
     // ---- softmax: a thread a row
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -583,7 +706,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
   float* xs = reinterpret_cast<float*>(ring);  // the second group's rows: O, then m and l
   const bool recompute = *odd != 0;
-  if (!failed && !recompute && warp >= 4) {
+  if (!failed && !recompute && warp >= 4 && warp < 12) {
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     float* xr = xs + (size_t)row * W::XROW;
     float* xml = xs + (size_t)kRows * W::XROW + row * 2;
@@ -669,10 +792,15 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     // Key by key over what each row sees: a warp a row, HD / 32 dims a lane.
     constexpr int DPL = HD / 32;
     const int32_t* table = p.tables + (size_t)b * p.table_stride;
-    const __nv_bfloat16* pk = static_cast<const __nv_bfloat16*>(p.pool_k);
-    const __nv_bfloat16* pv = static_cast<const __nv_bfloat16*>(p.pool_v);
+    auto element = [&](const void* pool, const uint8_t* scales, size_t row, int d) {
+      if constexpr (FP8) {
+        return scale_value(scales[row]) * __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(pool)[row * HD + d], __NV_E4M3)));
+      } else {
+        return __bfloat162float(static_cast<const __nv_bfloat16*>(pool)[row * HD + d]);
+      }
+    };
     const float sl = p.scale * 1.4426950408889634f;
-    for (int r = warp; r < rows; r += kThreads / 32) {
+    for (int r = warp; r < rows; r += threads_of(FP8) / 32) {
       const int node = node_of(p, row0 + r);
       const uint32_t* mask = p.mask ? p.mask + (size_t)(qoff + node) * p.mask_words : nullptr;
       float qv[DPL], acc[DPL] = {};
@@ -684,10 +812,10 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (j >= 0 && !(mask ? mask_bits<1>(mask, p.mask_words, j) & 1u : j <= node)) continue;
         const int blk = table[key / p.bs];
         const bool in = blk >= 0 && blk < p.num_blocks;  // reported by the loader
-        const size_t at = in ? (((size_t)blk * p.bs + key % p.bs) * p.nkv + h) * HD : 0;
+        const size_t at = in ? ((size_t)blk * p.bs + key % p.bs) * p.nkv + h : 0;
         float s = 0.f;
 #pragma unroll
-        for (int d = 0; d < DPL; ++d) s += in ? qv[d] * __bfloat162float(pk[at + lane + 32 * d]) : 0.f;
+        for (int d = 0; d < DPL; ++d) s += in ? qv[d] * element(p.pool_k, p.k_scale, at, lane + 32 * d) : 0.f;
         s = warp_sum(s) * sl;
         if (s > rm) {
           const float f = ex2(rm - s);
@@ -700,7 +828,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         rl += e;
 #pragma unroll
         for (int d = 0; d < DPL; ++d)
-          if (e != 0.f) acc[d] += in ? e * __bfloat162float(pv[at + lane + 32 * d]) : 0.f;
+          if (e != 0.f) acc[d] += in ? e * element(p.pool_v, p.v_scale, at, lane + 32 * d) : 0.f;
       }
 #pragma unroll
       for (int d = 0; d < DPL; ++d) {
@@ -729,7 +857,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   __syncthreads();
   if (!*last || failed) return;
   __threadfence();
-  for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
+  for (int i = threadIdx.x; i < rows * (HD / 4); i += threads_of(FP8)) {
     const int r = i / (HD / 4), d = i % (HD / 4) * 4;
     const float* pr = part0 + (size_t)r * PROW;
     float rm = -INFINITY, rl = 0.f;
@@ -804,7 +932,7 @@ bool pool_map(CUtensorMap* map, const void* pool, int64_t rows, int width, int h
   });
 }
 
-template <int HD, bool TWO>
+template <int HD, bool TWO, bool FP8>
 int launch(const TreeParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int batch, cudaStream_t stream) {
   using W = WideShape<HD, TWO>;
   static std::atomic<uint64_t> prepared{0};  // the shared-memory limit is an attribute of the kernel on one device
@@ -812,14 +940,14 @@ int launch(const TreeParams& p, const CUtensorMap& mk, const CUtensorMap& mv, in
   cudaError_t err = cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (err == cudaSuccess && !(prepared.load(std::memory_order_relaxed) & bit)) {
-    err = cudaFuncSetAttribute(tree_attn_wide_kernel<HD, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W::SMEM);
+    err = cudaFuncSetAttribute(tree_attn_wide_kernel<HD, TWO, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W::SMEM);
     if (err == cudaSuccess) prepared.fetch_or(bit, std::memory_order_relaxed);
   }
   if (err != cudaSuccess) {
     cudaGetLastError();
     return set_error(KVE_ERR_CUDA, "kve_paged_tree_attn: %s", cudaGetErrorString(err));
   }
-  launch_kernel(tree_attn_wide_kernel<HD, TWO>, dim3(batch * p.nkv, p.n_chunks, p.n_qtiles), dim3(kThreads), W::SMEM, stream,
+  launch_kernel(tree_attn_wide_kernel<HD, TWO, FP8>, dim3(batch * p.nkv, p.n_chunks, p.n_qtiles), dim3(threads_of(FP8)), W::SMEM, stream,
                 mk, mv, p);
   return check_launch("kve_paged_tree_attn(wide)");
 }
@@ -832,7 +960,7 @@ size_t tree_attn_wide_partial_bytes(int batch, int max_q, int max_ctx, int nkv, 
   return (size_t)batch * nkv * w.n_qtiles * w.n_chunks * ((w.two ? 2 : 1) * kRows) * (hd + 4) * sizeof(float);
 }
 
-int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, cudaStream_t stream) {
+int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, bool fp8, cudaStream_t stream) {
   const WidePlan w = wide_plan(batch, p.max_q, max_ctx, p.nkv, p.group);
   p.chunk = w.chunk;
   p.n_chunks = w.n_chunks;
@@ -841,10 +969,14 @@ int tree_attn_wide(TreeParams p, int batch, int max_ctx, int hd, cudaStream_t st
   memset(&mk, 0, sizeof(mk));
   memset(&mv, 0, sizeof(mv));
   const int64_t rows = p.num_blocks * p.bs;
-  if (!pool_map(&mk, p.pool_k, rows, p.nkv * hd, hd, false) || !pool_map(&mv, p.pool_v, rows, p.nkv * hd, hd, true))
+  if (!fp8 && (!pool_map(&mk, p.pool_k, rows, p.nkv * hd, hd, false) || !pool_map(&mv, p.pool_v, rows, p.nkv * hd, hd, true)))
     return set_error(KVE_ERR_CUDA, "kve_paged_tree_attn: no tensor map for the pool");
-  if (hd == 64) return w.two ? launch<64, true>(p, mk, mv, batch, stream) : launch<64, false>(p, mk, mv, batch, stream);
-  return w.two ? launch<128, true>(p, mk, mv, batch, stream) : launch<128, false>(p, mk, mv, batch, stream);
+  auto go = [&](auto f) {
+    constexpr bool F = decltype(f)::value;
+    if (hd == 64) return w.two ? launch<64, true, F>(p, mk, mv, batch, stream) : launch<64, false, F>(p, mk, mv, batch, stream);
+    return w.two ? launch<128, true, F>(p, mk, mv, batch, stream) : launch<128, false, F>(p, mk, mv, batch, stream);
+  };
+  return fp8 ? go(std::true_type()) : go(std::false_type());
 }
 
 }  // namespace kve

@@ -153,7 +153,9 @@ def test_tree_attention_long_histories_are_split_and_joined(cuda_device, cache, 
     assert torch.equal(ops.tree_attention(**args, workspace=ws), got)
 
 
-@pytest.mark.parametrize("heads", [(14, 2, 64), (16, 2, 128), (3, 3, 64), (64, 1, 128)])
+@pytest.mark.parametrize("cache, heads", [("bf16", (14, 2, 64)), ("bf16", (16, 2, 128)), ("bf16", (3, 3, 64)),
+                                          ("bf16", (64, 1, 128)), ("fp8", (14, 2, 64)), ("fp8", (16, 2, 128)),
+                                          ("fp8", (3, 3, 64))])
 @pytest.mark.parametrize("nodes, hists, bs, kind", [
     ([45], [0], 16, "tree"),                     # the tree alone
     ([50, 64, 7], [300, 129, 128], 16, "tree"),  # histories around a key tile's end
@@ -161,9 +163,9 @@ def test_tree_attention_long_histories_are_split_and_joined(cuda_device, cache, 
     ([64, 64], [63, 1000], 48, "none"),          # chains
     ([33, 0, 35], [2500, 5, 90], 16, "tree"),    # split into chunks, a sequence without new tokens
 ])
-def test_tree_attention_many_rows(cuda_device, heads, nodes, hists, bs, kind):
+def test_tree_attention_many_rows(cuda_device, cache, heads, nodes, hists, bs, kind):
     """Trees of more rows than one tensor-core tile, in every arrangement of tiles and chunks."""
-    args, *lens = attention_case("bf16", heads, nodes, hists, bs, kind, 17, cuda_device)
+    args, *lens = attention_case(cache, heads, nodes, hists, bs, kind, 17, cuda_device)
     status = ops.status_tensor(cuda_device)
     ws = ops.Workspace(cuda_device)
     got = ops.tree_attention(**args, workspace=ws, status=status)
@@ -171,6 +173,17 @@ def test_tree_attention_many_rows(cuda_device, heads, nodes, hists, bs, kind):
     assert int(status) == 0 and int(ws.buf[:65536].view(torch.int32).abs().sum()) == 0
     assert torch.equal(ops.tree_attention(**args, workspace=ws), got)
     check_attention(dict(args, scale=-0.05), *lens, ops.tree_attention(**dict(args, scale=-0.05)))
+
+
+@pytest.mark.parametrize("heads, nodes", [((8, 4, 64), 8), ((16, 4, 128), 40)])
+@pytest.mark.parametrize("cache", ["bf16", "fp8"])
+def test_tree_attention_long_chunks(cuda_device, cache, heads, nodes):
+    """More sequences than the grid needs: a block's keys go round its ring several times."""
+    hists = [1400 + 13 * i % 200 for i in range(40)]
+    args, *lens = attention_case(cache, heads, [nodes] * 40, hists, 16, "tree", 29, cuda_device)
+    status = ops.status_tensor(cuda_device)
+    check_attention(args, *lens, ops.tree_attention(**args, status=status))
+    assert int(status) == 0
 
 
 def test_tree_attention_joins_with_extreme_scores(cuda_device):
@@ -224,7 +237,7 @@ def test_tree_attention_few_rows_bad_block(cuda_device):
         check_attention(zero, ctx, nodes, off, got)
 
 
-@pytest.mark.parametrize("heads", [(4, 2, 64), (4, 4, 64), (2, 2, 128)])
+@pytest.mark.parametrize("heads", [(4, 2, 64), (4, 4, 64), (2, 2, 128), (16, 2, 128)])
 @pytest.mark.parametrize("cache", ["bf16", "fp32", "fp8"])
 def test_tree_attention_garbage_in_unseen_places(cuda_device, cache, heads):
     """Infinities and NaN in unused slots, in a partial page's tail and in nodes a row does not see
