@@ -412,6 +412,10 @@ tree_attn_kernel(TreeParams p) {
           sc[j][2 + e] *= k2;
         }
     } else {
+      // The tensor cores truncate what they add up: every 16 dims start from zero and are added
+      // here, rounded, and the products with a low half have sums of their own (one running sum
+      // for all was off by 1.3e-6 of the output at 131 keys, these by 1.9e-7).
+      float low[2][4] = {};
 #pragma unroll
       for (int k16 = 0; k16 < HD / 16; ++k16) {
         // dims 16 k16 + 4 tq .. + 3 of this lane: step s takes 2 s and 2 s + 1 of them
@@ -431,18 +435,25 @@ tree_attn_kernel(TreeParams p) {
           split_tf32(__uint_as_float(x.y), kh[1], kl[1]);
           split_tf32(__uint_as_float(x.z), kh[2], kl[2]);
           split_tf32(__uint_as_float(x.w), kh[3], kl[3]);
+          float part[4] = {};
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const uint32_t ah[4] = {s ? qh[0].z : qh[0].x, s ? qh[1].z : qh[1].x, s ? qh[0].w : qh[0].y,
                                     s ? qh[1].w : qh[1].y};
             const uint32_t al[4] = {s ? qlo[0].z : qlo[0].x, s ? qlo[1].z : qlo[1].x, s ? qlo[0].w : qlo[0].y,
                                     s ? qlo[1].w : qlo[1].y};
-            mma_tf32(sc[j], al, kh[2 * s], kh[2 * s + 1]);
-            mma_tf32(sc[j], ah, kl[2 * s], kl[2 * s + 1]);
-            mma_tf32(sc[j], ah, kh[2 * s], kh[2 * s + 1]);
+            mma_tf32(low[j], al, kh[2 * s], kh[2 * s + 1]);
+            mma_tf32(low[j], ah, kl[2 * s], kl[2 * s + 1]);
+            mma_tf32(part, ah, kh[2 * s], kh[2 * s + 1]);
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] += part[e];
         }
       }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[j][e] += low[j][e];
     }
 
     // Which of the tile's keys the two rows see.
@@ -531,27 +542,36 @@ tree_attn_kernel(TreeParams p) {
           }
       }
     } else if constexpr (KV == kF32) {
+      // k8 step j: lane position tq stands for key 2 tq, tq + 4 for key 2 tq + 1
+      uint32_t ph[2][4], pl[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        // k8 step j: lane position tq stands for key 2 tq, tq + 4 for key 2 tq + 1
-        uint32_t ph[4], pl[4];
-        split_tf32(sc[j][0], ph[0], pl[0]);
-        split_tf32(sc[j][2], ph[1], pl[1]);
-        split_tf32(sc[j][1], ph[2], pl[2]);
-        split_tf32(sc[j][3], ph[3], pl[3]);
-        const int k0 = 8 * j + 2 * tq;
+        split_tf32(sc[j][0], ph[j][0], pl[j][0]);
+        split_tf32(sc[j][2], ph[j][1], pl[j][1]);
+        split_tf32(sc[j][1], ph[j][2], pl[j][2]);
+        split_tf32(sc[j][3], ph[j][3], pl[j][3]);
+      }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const int piece = d * 2 + (g >> 2);
-          const float x0 = __uint_as_float(lds32(vb + k0 * ROWB + swz<KV, CH>(k0, piece) * 16 + (g & 3) * 4));
-          const float x1 = __uint_as_float(lds32(vb + (k0 + 1) * ROWB + swz<KV, CH>(k0 + 1, piece) * 16 + (g & 3) * 4));
-          uint32_t h0, l0, h1, l1;
-          split_tf32(x0, h0, l0);
-          split_tf32(x1, h1, l1);
-          mma_tf32(acc[d], pl, h0, h1);
-          mma_tf32(acc[d], ph, l0, l1);
-          mma_tf32(acc[d], ph, h0, h1);
+      for (int d = 0; d < DT; ++d) {
+        const int piece = d * 2 + (g >> 2);
+        uint32_t vh[2][2], vl[2][2];
+        float part[4] = {};  // the tile's sum, added to the others rounded
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = 8 * j + 2 * tq + e;
+            split_tf32(__uint_as_float(lds32(vb + key * ROWB + swz<KV, CH>(key, piece) * 16 + (g & 3) * 4)), vh[j][e], vl[j][e]);
+          }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mma_tf32(part, pl[j], vh[j][0], vh[j][1]);
+          mma_tf32(part, ph[j], vl[j][0], vl[j][1]);
         }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma_tf32(part, ph[j], vh[j][0], vh[j][1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[d][e] += part[e];
       }
     } else {
       uint32_t pa[4];
