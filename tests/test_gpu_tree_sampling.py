@@ -186,6 +186,30 @@ def test_tree_attention_long_chunks(cuda_device, cache, heads, nodes):
     assert int(status) == 0
 
 
+@pytest.mark.parametrize("bs", [16, 7])
+@pytest.mark.parametrize("exponent", [30, 127, 134, 135, 150])
+@pytest.mark.parametrize("group", [1, 16])
+def test_tree_attention_over_one_8_bit_key_is_its_value(cuda_device, group, exponent, bs):
+    """One key: p = 1, and every finite e4m3 times 2^(exponent - 127) is a bf16: the output is V exactly, NaN bytes NaN."""
+    pool_k = torch.zeros(4, bs, 2, 128, dtype=torch.uint8, device=cuda_device)
+    pool_v = (torch.arange(4 * bs * 2 * 128, device=cuda_device) * 37 % 256).to(torch.uint8).view(4, bs, 2, 128)
+    scale = torch.full((4, bs, 2), exponent, dtype=torch.uint8, device=cuda_device)
+    for history in (False, True):  # the key is the new token, or of the history (and the new token unseen)
+        ctx = 2 if history else 1
+        mask = torch.ones(2, 1, dtype=torch.int32, device=cuda_device) * (0 if history else 1)
+        if history:
+            pool_v[2, 1] = 0
+        out = ops.tree_attention(
+            torch.ones(1, 2 * group, 128, dtype=torch.bfloat16, device=cuda_device), pool_k.view(torch.float8_e4m3fn),
+            pool_v.view(torch.float8_e4m3fn), torch.tensor([[2]], dtype=torch.int32, device=cuda_device),
+            *[torch.tensor([x], dtype=torch.int32, device=cuda_device) for x in (ctx, 1, 0)], 1, ctx, 0.1,
+            tree_mask=mask[:1], k_scale=scale, v_scale=scale)
+        want = pool_v[2, 0].view(torch.float8_e4m3fn).float() * 2.0 ** (exponent - 127)
+        assert bool(want.isnan().any())
+        got = out.float().view(2, group, 128)
+        assert torch.equal(got.nan_to_num(7e30), want.nan_to_num(7e30)[:, None].expand(2, group, 128)), (group, exponent, history)
+
+
 def test_tree_attention_joins_with_extreme_scores(cuda_device):
     """Scores hundreds apart between chunks and streams: shares of exactly 0 and 1, no overflow."""
     for cache in ("bf16", "fp32", "fp8"):
