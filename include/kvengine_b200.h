@@ -380,9 +380,9 @@ int kve_spec_next_draft_plan(const int32_t* start_lens, const int32_t* last_toke
  * bf16 queries over a cache written by the *_fp8 ops, with the layer's scale bytes
  * [num_blocks, block_size, num_kv_heads]. q, out, tables, lengths and offsets as
  * for kve_paged_verify_attn; head_dim 64 or 128, at most 64 query heads per kv head,
- * max_q_len <= 1024 (longer prompts: in pieces), ctx_lens[b] <= max_ctx.
- * Only the rows [q_offsets[b], q_offsets[b] + q_lens[b]) of out are written.
- * A sequence with inconsistent lengths is skipped, a block id outside the pool reads
+ * max_q_len <= 1024 (longer prompts: in pieces), ctx_lens[b] <= max_ctx, scale finite.
+ * q, out and tree_mask have q_rows rows; only [q_offsets[b], q_offsets[b] + q_lens[b]) of out are
+ * written. A sequence with inconsistent lengths, or rows past q_rows, is skipped, a block id outside the pool reads
  * as zeros; both record KVE_ERR_BOUNDS. Workspace: zeroed once; as
  * kve_tree_attn_workspace_bytes says (0: none). */
 size_t kve_tree_attn_workspace_bytes(int batch, int max_q_len, int max_ctx, int num_heads, int num_kv_heads,
@@ -390,9 +390,9 @@ size_t kve_tree_attn_workspace_bytes(int batch, int max_q_len, int max_ctx, int 
 int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k, const void* pool_v, int kv_dtype,
                         const uint8_t* k_scale, const uint8_t* v_scale, const int32_t* block_tables, int table_stride,
                         const int32_t* ctx_lens, const int32_t* q_lens, const int32_t* q_offsets,
-                        const uint32_t* tree_mask, int mask_words, int batch, int max_q_len, int max_ctx, int num_heads,
-                        int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, float scale, void* out,
-                        void* workspace, size_t workspace_bytes, int* dev_status, cudaStream_t stream);
+                        const uint32_t* tree_mask, int mask_words, int batch, int q_rows, int max_q_len, int max_ctx,
+                        int num_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, float scale,
+                        void* out, void* workspace, size_t workspace_bytes, int* dev_status, cudaStream_t stream);
 
 /* The 8-bit cache. A row (token, kv head, K or V) of head_dim (64 or 128) elements x is
  * held as e4m3 numbers q = x 2^-e rounded to nearest even, and the byte e + 127,

@@ -96,7 +96,7 @@ _SIGNATURES = {
     "kve_forward_layers_graphed": (i32, [C.POINTER(ModelT), C.POINTER(BatchT), C.POINTER(ScratchT), i32, i32,
                                          C.POINTER(C.c_void_p), vp]),
     "kve_tree_attn_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
-    "kve_paged_tree_attn": (i32, [vp, i32, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32,
+    "kve_paged_tree_attn": (i32, [vp, i32, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
                                   i32, i32, i64, f32, vp, vp, sz, vp, vp]),
     "kve_qkv_rope_append_fp8": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, i64, vp,
                                       vp]),

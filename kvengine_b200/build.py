@@ -80,6 +80,8 @@ def build_fastcall(force: bool = False, verbose: bool = False) -> str:
     src = os.path.join(CSRC, "fastcall.cpp")
     if not force and _newer(FAST, [src, os.path.join(INCLUDE, "kvengine_b200.h")]):
         return FAST
+    if os.path.exists(FAST):  # one built for an older header would pass other arguments
+        os.remove(FAST)
     home = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
     cmd = [os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",

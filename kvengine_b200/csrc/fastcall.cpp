@@ -189,8 +189,8 @@ PyObject* tree_attention(PyObject* const* a) {
   }
   const int rc = f_tree_attn(q.data_ptr(), code, k.data_ptr(), v.data_ptr(), kv_code, ks, vs, at_ptr<int32_t>(tables),
                              (int)tables.size(1), at_ptr<int32_t>(ctx), at_ptr<int32_t>(ql), at_ptr<int32_t>(qo), mask, words,
-                             (int)B, max_q, max_ctx, (int)nq, (int)k.size(2), (int)hd, (int)k.size(1), k.size(0), (float)scale,
-                             out.data_ptr(), ws, size, status, stream(dev));
+                             (int)B, (int)q.size(0), max_q, max_ctx, (int)nq, (int)k.size(2), (int)hd, (int)k.size(1), k.size(0),
+                             (float)scale, out.data_ptr(), ws, size, status, stream(dev));
   return result(rc, single, &out);
 }
 

@@ -24,7 +24,7 @@ struct TreeParams {
   const int32_t* q_offsets;
   const uint32_t* mask;
   int mask_words;
-  int max_q, nq, nkv, group, bs;
+  int q_rows, max_q, nq, nkv, group, bs;
   int64_t num_blocks;
   float scale;
   void* out;

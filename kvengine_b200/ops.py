@@ -303,8 +303,9 @@ def tree_attention(q, pool_k_layer, pool_v_layer, block_tables, ctx_lens, q_lens
     """Attention of drafted trees over a paged cache (kve_paged_tree_attn). Arguments as for
     `paged_attention`; tree_mask [sum q_lens, words] int32: bit t % 32 of word t / 32 of a row says
     whether it sees node t of its sequence (`tree_mask_words` builds it from parents; None: a
-    chain); a row that sees nothing gets zeros. bf16 queries also read an e4m3 cache, given
-    its layer's k_scale and v_scale [num_blocks, bs, nkv] uint8."""
+    chain); a row that sees nothing gets zeros, rows of `out` of no sequence are left as they are.
+    bf16 queries also read an e4m3 cache, given its layer's k_scale and v_scale [num_blocks, bs,
+    nkv] uint8."""
     r = L.fast().tree_attention(q, pool_k_layer, pool_v_layer, block_tables, ctx_lens, q_lens, q_offsets, max_q_len,
                                 max_ctx, scale, tree_mask, k_scale, v_scale, out,
                                 None if workspace is None else workspace.buf, status)
@@ -353,7 +354,7 @@ def tree_attention(q, pool_k_layer, pool_v_layer, block_tables, ctx_lens, q_lens
         buf = (workspace or Workspace(q.device)).get(need)
         ws, ws_bytes = buf.data_ptr(), buf.numel()
     _call(lib.kve_paged_tree_attn, dev, q.data_ptr(), code, pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), kv_code, ks, vs,
-          block_tables.data_ptr(), width, ctx_lens.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(), mask, words, B,
+          block_tables.data_ptr(), width, ctx_lens.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(), mask, words, B, n,
           max_q_len, max_ctx, nq, nkv, hd, bs, num_blocks, scale, out.data_ptr(), ws, ws_bytes, L.ptr(status))
     return out
 

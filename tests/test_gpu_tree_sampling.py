@@ -12,7 +12,9 @@ over the row's keys):
   * bf16 rounds p (u16 A) and the output (u16 |o|); fp32 splits p and v to 2^-22 each (2^-21 A, the
     same again for q and k: 2^-21 s in d) and rounds the output (u32 |o|);
   * sums of up to n terms in fp32: n u32 A, n < 2^12 here, in chains far shorter: 2^-14 A is generous for
-    bf16 (a sixty-fourth of u16 A); fp32 sums its n terms in order within a stream: n u32 A.
+    bf16 (a sixty-fourth of u16 A; where more than eight rows share a kv head, a quarter of the
+    exponentials come from a polynomial off by 2.6e-6 of the value, 2^-18, well inside it); fp32
+    sums its n terms in order within a stream: n u32 A.
 log-probabilities: (x - m) / T - log z with z from ex2.approx (2^-22 relative, arguments in fp32 off by
 2 u32 |x - m| / T) and sums of a few dozen fp32 additions (64 u32): in absolute terms
 2^-22 + 2 u32 R + 64 u32, R the range of (x - m) / T that carries weight (below 40), then one rounding.
@@ -25,6 +27,7 @@ import pytest
 import torch
 
 from kvengine_b200 import PagedKVCache, ops
+from kvengine_b200 import _lib as L
 
 pytestmark = pytest.mark.gpu
 U16, U32 = torch.finfo(torch.bfloat16).eps / 2, torch.finfo(torch.float32).eps / 2
@@ -323,6 +326,40 @@ def test_tree_attention_value_seen_with_an_infinity(cuda_device, cache):
     assert bool(((got - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("nodes", [1, 9, 40])
+@pytest.mark.parametrize("cache", ["bf16", "fp32", "fp8"])
+def test_tree_attention_nan_and_infinite_scores_in_the_history(cuda_device, cache, nodes):
+    """Every row sees the history: a NaN there, or an infinite score, makes its kv head's rows NaN, whichever key
+    of a tile it is, and no other's."""
+    args, *_ = attention_case(cache, (8, 2, 64), [nodes], [330], 16, "tree", 37, cuda_device)
+    want = ops.tree_attention(**args)[:nodes]
+    bits = {"bf16": torch.int16, "fp32": torch.int32, "fp8": torch.uint8}[cache]
+    nan = torch.tensor(math.nan).to(args["pool_k_layer"].dtype).view(bits).to(cuda_device)
+    table = args["block_tables"][0].tolist()
+    for which in ("pool_k_layer", "pool_v_layer"):
+        for pos in list(range(8)) + [62, 63, 64, 127, 190, 319]:
+            pool = args[which].view(bits).clone()
+            pool[table[pos // 16], pos % 16, 0, :] = nan
+            got = ops.tree_attention(**dict(args, **{which: pool.view(args[which].dtype)}))[:nodes]
+            assert bool(got[:, :4].isnan().all()), (which, pos)
+            assert torch.equal(got[:, 4:], want[:, 4:]), (which, pos)
+    if cache == "bf16":  # q.k overflows fp32 for one key
+        for pos in (6, 7, 70, 200):
+            pool = args["pool_k_layer"].clone()
+            pool[table[pos // 16], pos % 16, 0, :] = 3e38 * args["q"][0, 0].sign()
+            got = ops.tree_attention(**dict(args, q=args["q"][:1].expand(nodes, -1, -1)[:, :1].expand(-1, 8, -1).contiguous(),
+                                            tree_mask=args["tree_mask"][:nodes], pool_k_layer=pool))
+            assert bool(got[:, :4].isnan().all()) and bool(got[:, 4:].isfinite().all()), pos
+
+
+@pytest.mark.parametrize("nodes", [1, 9, 40])
+@pytest.mark.parametrize("cache", ["bf16", "fp32", "fp8"])
+def test_tree_attention_with_scale_zero_is_the_mean(cuda_device, cache, nodes):
+    args, *lens = attention_case(cache, (8, 2, 64), [nodes, nodes], [100, 0], 16, "random", 41, cuda_device)
+    args["scale"] = 0.0
+    check_attention(args, *lens, ops.tree_attention(**args))
+
+
 def test_tree_attention_leaves_other_rows_and_reports_bad_inputs(cuda_device):
     dev = cuda_device
     args, ctx, nodes, off = attention_case("bf16", (4, 2, 64), [3, 2, 4], [30, 17, 9], 16, "tree", 9, dev)
@@ -347,6 +384,27 @@ def test_tree_attention_leaves_other_rows_and_reports_bad_inputs(cuda_device):
     tables[2, 0] = 1 << 20
     got = ops.tree_attention(**dict(args, block_tables=tables), status=status)
     assert int(status) == -7 and torch.equal(got[:5], want[:5]) and torch.isfinite(got[:9].float()).all()
+
+
+@pytest.mark.parametrize("cache, heads, nodes", [("bf16", (4, 2, 64), [2, 2, 1]), ("fp8", (4, 2, 64), [2, 2, 1]),
+                                                 ("bf16", (8, 2, 128), [9, 9, 4]), ("fp8", (8, 2, 128), [9, 9, 4]),
+                                                 ("fp32", (4, 2, 64), [5, 5, 3])])
+def test_tree_attention_rows_past_the_end_are_refused(cuda_device, cache, heads, nodes):
+    """An offset that would put a sequence's rows past q's: skipped and reported; the others are right."""
+    args, *_ = attention_case(cache, heads, nodes, [50, 20, 90], 16, "tree", 31, cuda_device)
+    rows = sum(nodes)
+    for key, short in (("q", rows), ("tree_mask", rows)):
+        args[key] = args[key][:short].contiguous()
+    want = ops.tree_attention(**args)
+    for bad in (rows - nodes[1] + 1, rows, 2 ** 31 - 1, -1):
+        status = ops.status_tensor(cuda_device)
+        off = args["q_offsets"].clone()
+        off[1] = bad
+        out = torch.full_like(want, 7.0)
+        ops.tree_attention(**dict(args, q_offsets=off), out=out, status=status)
+        assert int(status) == -7, bad
+        a, b = nodes[0], nodes[0] + nodes[1]
+        assert torch.equal(out[:a], want[:a]) and torch.equal(out[b:], want[b:]) and bool((out[a:b] == 7).all()), bad
 
 
 def test_tree_attention_far_offsets(cuda_device):
@@ -999,3 +1057,18 @@ def test_a_tree_step_then_a_decode_step(cuda_device, cache):
             q = append(p, layer, step[layer], kept, [s.slot_list(keep, 1)[0] for s, keep in zip(ss, kept)])
             outs.append(attend(p, layer, q, ss, [keep + 1 for keep in kept], [1, 1], None)[1])
         assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("cache", ["bf16", "fp8"])
+def test_calls_without_the_cpp_binding(cuda_device, monkeypatch, cache):
+    """The same calls through Python and ctypes: results, checks and refusals."""
+    monkeypatch.setattr(L, "_fast", L._NoFast())
+    test_tree_attention_many_rows(cuda_device, cache, (16, 2, 128), [8, 3], [100, 700], 16, "tree")
+    test_tree_attention_wrapper_refusals(cuda_device)
+    test_kv_append_and_read_fp8(cuda_device, torch.bfloat16, 2, 64, 16, 67)
+    test_qkv_rope_append_fp8(cuda_device, torch.float32, 14, 2, 64, 5)
+    test_sample_accept(cuda_device, torch.bfloat16, 5, 4, 1000, True)
+    test_tree_sample_accept(cuda_device, torch.float32, 1024, [7, 33, 0, 2])
+    test_sampling_wrapper_refusals(cuda_device)
+    test_kv_commit_path(cuda_device, cache, 2, 64, 16, 3)
+    test_a_tree_step_then_a_decode_step(cuda_device, cache)

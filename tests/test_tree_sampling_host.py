@@ -21,12 +21,13 @@ def refused(code, words, rc):
 
 
 ATTN = dict(q=P, dtype=L.KVE_BF16, pool_k=P, pool_v=P, kv_dtype=L.KVE_BF16, k_scale=None, v_scale=None, tables=P, stride=8,
-            ctx=P, q_lens=P, q_offsets=P, mask=P, words=1, batch=2, max_q=9, max_ctx=100, nq=8, nkv=2, hd=64, bs=16,
+            ctx=P, q_lens=P, q_offsets=P, mask=P, words=1, batch=2, q_rows=18, max_q=9, max_ctx=100, nq=8, nkv=2, hd=64, bs=16,
             blocks=32, scale=0.1, out=P, ws=P, ws_bytes=1 << 30, status=None, stream=None)
 
 
 @pytest.mark.parametrize("change, code, words", [
-    (dict(batch=-1), -1, "bad sizes"), (dict(max_q=-1), -1, "bad sizes"), (dict(max_ctx=8), -1, "bad sizes"),
+    (dict(batch=-1), -1, "bad sizes"), (dict(max_q=-1), -1, "bad sizes"), (dict(q_rows=-1), -1, "bad sizes"), (dict(scale=float("nan")), -1, "scale nan"),
+    (dict(scale=float("inf")), -1, "scale inf"), (dict(max_ctx=8), -1, "bad sizes"),
     (dict(nq=7), -1, "bad sizes"), (dict(nkv=0), -1, "bad sizes"), (dict(bs=0), -1, "bad sizes"),
     (dict(stride=0), -1, "bad sizes"), (dict(blocks=0), -1, "bad sizes"),
     (dict(hd=96), -2, "head_dim 96"), (dict(nq=130), -2, "group 65"),
@@ -175,3 +176,14 @@ def test_fp8_pool_bookkeeping():
     assert pool.nbytes() == 2 * (2 * 8 * 16 * 2 * 64 + 2 * 8 * 16 * 2)
     assert int(pool.k_scale.min()) == int(pool.v_scale.max()) == 127
     assert PagedKVCache(2, 2, 64, 8, 16, torch.bfloat16, "cpu").k_scale is None
+
+
+def test_the_cpp_binding_is_built_and_leaves_other_calls_to_python():
+    """Its functions return None, and touch nothing, for what is not a CUDA tensor."""
+    fast = L.fast()
+    assert not isinstance(fast, L._NoFast)
+    q = torch.zeros(1, 2, 64)
+    i = torch.zeros(1, dtype=torch.int32)
+    assert fast.tree_attention(q, q, q, i, i, i, i, 1, 1, 1.0, None, None, None, None, None, None) is None
+    with pytest.raises((ValueError, RuntimeError, TypeError)):
+        ops.tree_attention(q, q[None], q[None], i[None], i, i, i, 1, 1, 1.0)
