@@ -366,83 +366,114 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   // e4m3: two warps copy K and two V, 32 of a tile's keys each, through their registers into the places
   // where TMA puts bf16 tiles, as the bf16 numbers they stand for. The bytes are asked for two tiles
   // ahead. (One warp for all of K or V, one tile ahead, took 8000 cycles a tile.)
-  auto copy_fp8 = [&](bool v, int half) {
+  auto copy_fp8 = [&](auto is_v, int half) {
+    constexpr bool v = decltype(is_v)::value;
     constexpr int PIECES = HD / 16, PER = PIECES;  // 16-byte pieces of a key; a lane's, of a tile
     constexpr int AT_ONCE = 32 / PIECES;           // keys of one load
     const uint8_t* pool = static_cast<const uint8_t*>(v ? p.pool_v : p.pool_k) + (size_t)h * HD + lane % PIECES * 16;
     const uint8_t* scales = (v ? p.v_scale : p.k_scale) + h;
     const int32_t* table = p.tables + (size_t)b * p.table_stride;
+    const uint32_t row_bytes = (uint32_t)(p.nkv * HD);
+    // Where the lane's pieces go in a slot: load u's key is AT_ONCE u further, its two halves (8 elements
+    // each) in the columns that the key's last three bits swizzle.
+    const int r0 = lane / PIECES, piece0 = lane % PIECES * 2;
+    const uint32_t place = (uint32_t)(v ? half * (32 * HD * 2) + piece0 / 8 * 2048 : piece0 / 8 * (kKeys * 128) + half * 4096) + r0 * 128;
     uint4 bytes[2][PER];
-    uint32_t valid[2], byte[2];  // bit u: piece u's key is there; the exponent of this lane's key
-    auto key_of = [&](int t) { return key_lo + t * kKeys + 32 * half + lane; };
-    auto id_of = [&](int t) { return t < n && key_of(t) < key_hi ? table[key_of(t) / p.bs] : -1; };
-    auto ask = [&](int t, int id, int at) {  // tile t's bytes and exponents, `id` its block
-      const int key = key_of(t);
+    uint32_t byte[2];  // the exponent of this lane's key
+    int slots[2];      // its slot in the pool (-1: the key is not there)
+    bool found = false;
+    // The key's block and place in it, for the tile whose block id is asked for.
+    int key = key_lo + 32 * half + lane, blk = key / p.bs, in = key - blk * p.bs;
+    const int step_blk = kKeys / p.bs, step_in = kKeys - step_blk * p.bs;
+    int id = -1, id_in = 0;
+    bool id_key = false;
+    auto ask_id = [&] {
+      id_key = key < key_hi;
+      id = id_key ? table[blk] : -1;
+      id_in = in;
+      key += kKeys;
+      blk += step_blk;
+      in += step_in;
+      if (in >= p.bs) {
+        in -= p.bs;
+        ++blk;
+      }
+    };
+    auto ask = [&](int at) {  // the bytes and exponents of the tile whose block ids have come
       int slot = -1;
       uint32_t e = 0;
-      if (key < key_hi) {
-        if (id >= 0 && id < p.num_blocks) {
-          slot = id * p.bs + key % p.bs;
-          e = scales[(size_t)slot * p.nkv];
-        } else if (!v) {
-          report(p.status, KVE_ERR_BOUNDS);  // reads as zeros
-        }
+      if (id >= 0 && id < p.num_blocks) {
+        slot = id * p.bs + id_in;
+        e = scales[(size_t)slot * p.nkv];
+      } else if (!v && id_key) {
+        report(p.status, KVE_ERR_BOUNDS);  // reads as zeros
       }
       byte[at] = e;
-      valid[at] = 0;
+      slots[at] = slot;
+      slot = max(slot, 0);
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
-        const int sl = __shfl_sync(0xffffffffu, slot, u * AT_ONCE + lane / PIECES);
-        valid[at] |= (sl >= 0 ? 1u : 0u) << u;
-        bytes[at][u] = *reinterpret_cast<const uint4*>(pool + (size_t)(uint32_t)max(sl, 0) * (uint32_t)(p.nkv * HD));
+        const uint32_t sl = __shfl_sync(0xffffffffu, slot, u * AT_ONCE + r0);
+        bytes[at][u] = *reinterpret_cast<const uint4*>(pool + (uint64_t)sl * row_bytes);
       }
+      ask_id();
     };
-    auto store = [&](uint8_t* to, int u, const uint32_t (&o)[8]) {
-      const int r = 32 * half + u * AT_ONCE + lane / PIECES;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int piece = lane % PIECES * 2 + j;  // of the row's 8-element pieces
-        const size_t at = v ? (size_t)(r / 16) * (16 * HD * 2) + piece / 8 * 2048 + r % 16 * 128
-                            : (size_t)(piece / 8) * (kKeys * 128) + r * 128;
-        *reinterpret_cast<uint4*>(to + at + ((piece % 8 ^ (r & 7)) << 4)) =
-            make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-      }
-    };
-    bool found = false;
-    int id = id_of(2);
-    ask(0, id_of(0), 0);
-    if (n > 1) ask(1, id_of(1), 1);
-    auto tile = [&](int t, int at) {  // `at`: t mod 2, known when compiled
-      uint4 now[PER];
+    ask_id();
+    ask(0);
+    if (n > 1) ask(1);
+    auto tile = [&](int t, auto which) {
+      constexpr int at = decltype(which)::value;  // t mod 2
+      const uint4(&now)[PER] = bytes[at];
       // A byte's exponent and mantissa, put where bf16 has the low bits of its exponent and
       // the top of its mantissa, are the number times 2^-120, subnormals included: one product
       // with 2^(e - 127 + 120) makes it the bf16 that it stands for. Not where that power
-      // is no bf16, nor for NaN bytes: such a tile goes through the conversions.
-      uint32_t odd_bytes = 0;
+      // is no bf16, nor for NaN bytes, nor where keys are missing: such a tile goes the slow way.
+      uint32_t nan = 0;
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
-        const uint32_t keep = valid[at] >> u & 1 ? ~0u : 0u;
-        now[u] = make_uint4(bytes[at][u].x & keep, bytes[at][u].y & keep, bytes[at][u].z & keep, bytes[at][u].w & keep);
-        odd_bytes |= ((now[u].x & 0x7f7f7f7fu) + 0x01010101u) | ((now[u].y & 0x7f7f7f7fu) + 0x01010101u) |
-                     ((now[u].z & 0x7f7f7f7fu) + 0x01010101u) | ((now[u].w & 0x7f7f7f7fu) + 0x01010101u);
+        nan |= ((now[u].x & 0x7f7f7f7fu) + 0x01010101u) | ((now[u].y & 0x7f7f7f7fu) + 0x01010101u);
+        nan |= ((now[u].z & 0x7f7f7f7fu) + 0x01010101u) | ((now[u].w & 0x7f7f7f7fu) + 0x01010101u);
       }
       const uint32_t e = byte[at];
-      if (t + 2 < n) {
-        ask(t + 2, id, at);
-        id = id_of(t + 3);
-      }
+      const int slot = slots[at];
       if (t >= NK) ok = ok && mbar_wait(smem_u32(&empty[slot_of(v, t)]), parity_of(t - NK), p.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
-      uint8_t* to = ring + (size_t)slot_of(v, t) * W::SLOT;
-      const bool plain = !__any_sync(0xffffffffu, (odd_bytes & 0x80808080u) != 0 || e > 134);
-      const uint32_t mine = plain ? ((e + 120) << 7) * 0x10001u : __float_as_uint(scale_value(e));
+      uint8_t* to = ring + (size_t)slot_of(v, t) * W::SLOT + place;
+      auto store = [&](int u, const uint32_t (&o)[8]) {
+        const int r = u * AT_ONCE;
+        uint8_t* dst = to + (v ? r / 16 * (16 * HD * 2) + r % 16 * 128 : r * 128);
 #pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        const uint32_t up = __shfl_sync(0xffffffffu, mine, u * AT_ONCE + lane / PIECES);
-        const uint32_t w[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
-        uint32_t o[8];
-        if (plain) {
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<uint4*>(dst + (((piece0 + j) % 8 ^ (r + r0 & 7)) << 4)) =
+              make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+      };
+      if (__any_sync(0xffffffffu, (nan & 0x80808080u) != 0 || e > 134 || slot < 0)) {
+        const float mine = scale_value(e);
+#pragma unroll 1
+        for (int u = 0; u < PER; ++u) {
+          const int from = u * AT_ONCE + r0;
+          const float up = __shfl_sync(0xffffffffu, mine, from);
+          const int sl = __shfl_sync(0xffffffffu, slot, from);
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (sl >= 0) x = *reinterpret_cast<const uint4*>(pool + (uint64_t)(uint32_t)sl * row_bytes);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (i % 2 * 16)), __NV_E4M3);
+            const float2 f = __half22float2(__half2(two));
+            o[i] = pack2(f.x * up, f.y * up);
+          }
+          store(u, o);
+        }
+      } else {
+        const uint32_t mine = ((e + 120) << 7) * 0x10001u;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          const uint32_t up = __shfl_sync(0xffffffffu, mine, u * AT_ONCE + r0);
+          const uint32_t w[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
+          uint32_t o[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint32_t x = __byte_perm(w[i / 2], 0, i % 2 ? 0x3424 : 0x1404);
@@ -450,36 +481,38 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             const __nv_bfloat162 z = __hmul2(reinterpret_cast<const __nv_bfloat162&>(y), reinterpret_cast<const __nv_bfloat162&>(up));
             o[i] = reinterpret_cast<const uint32_t&>(z);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (i % 2 * 16)), __NV_E4M3);
-            const float2 f = __half22float2(__half2(two));
-            o[i] = pack2(f.x * __uint_as_float(up), f.y * __uint_as_float(up));
-          }
-        }
-        store(to, u, o);
-        if (v && t >= special) {  // infinities and NaN in new tokens' rows
-          const int key = key_lo + t * kKeys + 32 * half + u * AT_ONCE + lane / PIECES;
-          if (key >= hist && key < key_hi) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) found |= odd_bits(o[i]);
-          }
+          store(u, o);
         }
       }
+      if (t + 2 < n) ask(at);
+      if (v && t >= special) {  // infinities and NaN in new tokens' rows: this lane's own pieces, as stored
+#pragma unroll 1
+        for (int u = 0; u < PER; ++u) {
+          const int r = u * AT_ONCE, at_key = key_lo + t * kKeys + 32 * half + r + r0;
+          const uint8_t* src = to + r / 16 * (16 * HD * 2) + r % 16 * 128;
+          if (at_key >= hist && at_key < key_hi) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint4 x = *reinterpret_cast<const uint4*>(src + (((piece0 + j) % 8 ^ (r + r0 & 7)) << 4));
+              found |= odd_bits(x.x) || odd_bits(x.y) || odd_bits(x.z) || odd_bits(x.w);
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, found) && lane == 0) *odd = 1;
+      }
       fence_proxy_async_smem();
-      if (__any_sync(0xffffffffu, found) && lane == 0) *odd = 1;
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(v && t >= special ? &ready[(t - special) % NK] : &full[slot_of(v, t)]));
     };
     for (int t = 0; t < n && ok; t += 2) {
-      tile(t, 0);
-      if (t + 1 < n && ok) tile(t + 1, 1);
+      tile(t, std::integral_constant<int, 0>());
+      if (t + 1 < n && ok) tile(t + 1, std::integral_constant<int, 1>());
     }
   };
   if (FP8 && (warp == 0 || warp >= 12)) {
     if constexpr (FP8) {
-      if (warp >= 12) copy_fp8(warp & 1, (warp >> 1) & 1);
+      if (warp >= 12 && (warp & 1)) copy_fp8(std::true_type(), (warp >> 1) & 1);
+      else if (warp >= 12) copy_fp8(std::false_type(), (warp >> 1) & 1);
     }
   } else if (warp == 0) {
     // ---- K: boxes of 16 keys x 64 dims
