@@ -31,8 +31,8 @@
 // are computed again, key by key.
 //
 // Measured, 16 / 2 heads of 128: 32 trees of 64 nodes at 4500 keys 80 us (950 TFLOP/s), 64 of 16 nodes
-// at 175 to 700 keys 14.4 us; over e4m3 caches 307 us (bound by the four warps' conversion) and,
-// at 700 keys, 49 us (78 and 707 us in the kernel of tree_attn.cu). The wide case is bound by
+// at 175 to 700 keys 14.4 us; over e4m3 caches 261 us (the copying warps' chains of loads, conversions and stores) and,
+// at 700 keys, 41 us (707 and 78 us in the kernel of tree_attn.cu). The wide case is bound by
 // the softmax warps' issue slots; running every kShare-th pair of exponentials on
 // the fp32 units takes 81.7 us at 4, 85.7 at 2, and 87.2 with none.
 #include <cuda_fp8.h>
@@ -364,8 +364,9 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     return y;
   };
   // e4m3: two warps copy K and two V, 32 of a tile's keys each, through their registers into the places
-  // where TMA puts bf16 tiles, as the bf16 numbers they stand for. The bytes are asked for two tiles
-  // ahead. (One warp for all of K or V, one tile ahead, took 8000 cycles a tile.)
+  // where TMA puts bf16 tiles, as the bf16 numbers they stand for; when a tile is written the next
+  // one's bytes are on their way and those after it are asked for. (One warp for all of K or V: 432 us where
+  // this takes 261; a third pair gains nothing, nor do loads that pass L1 by.)
   auto copy_fp8 = [&](auto is_v, int half) {
     constexpr bool v = decltype(is_v)::value;
     constexpr int PIECES = HD / 16, PER = PIECES;  // 16-byte pieces of a key; a lane's, of a tile
@@ -388,7 +389,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     int id = -1, id_in = 0;
     bool id_key = false;
     auto ask_id = [&] {
-      id_key = key < key_hi;
+      id_key = (uint32_t)key < (uint32_t)key_hi;  // past 2^31 is past the end
       id = id_key ? table[blk] : -1;
       id_in = in;
       key += kKeys;
