@@ -399,6 +399,7 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
   };
   float key = -INFINITY;
   int at = -1;
+  bool near = false;  // this thread passed over a column whose key was within kMargin of its best one's
   __syncthreads();
   if (p.z > 0.0) {
     const float c = kLog2e / t, lz = sh.lz, off = p.b == INFINITY ? 0.f : -p.b;
@@ -412,11 +413,14 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
         const float w = ex2(e) * sh.inv_zp - qw * sh.inv_zq;
         k = w > 0.f ? __log2f(w) + gv : -INFINITY;
       }
-      if (!(k > key)) return;
+      if (!(k > key - kMargin)) return;
       for (int j = 0; j < n_skip; ++j)
         if (skip[j] == v) return;
-      key = k;
-      at = v;
+      near = k < key + kMargin;
+      if (k > key) {
+        key = k;
+        at = v;
+      }
       if (ordered(k) > *bar) atomicMax(&sh.bar, ordered(k));
     };
     auto one = [&](float x, int v) {
@@ -457,19 +461,26 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
     }
     for (int j = head + nvec * N + threadIdx.x; j < hi; j += kDrawThreads) one(Elem<T>::to_f(row[j]), j);
   }
+  // Column v's key in 64 bits; NaN where its weight rounds to nothing there.
+  auto exact = [&](int v, float x) {
+    if (!qrow) return (p.b == INFINITY ? 0.0 : (double)x / t) + (double)gumbel[v];
+    const double w = probability(p, x, v, t) - probability(q, Elem<T>::to_f(qrow[v]), v, t);
+    return w > 0.0 ? log(w) + (double)gumbel[v] : (double)NAN;
+  };
   __syncthreads();
-  if (at >= 0 && key >= unordered(sh.bar) - kMargin) {
-    const float x = clean(Elem<T>::to_f(row[at]));
-    const double gv = gumbel[at];
-    double k = key * 0.6931471805599453;  // stands where the weight rounds to nothing in 64 bits
-    if (qrow) {
-      const double w = probability(p, x, at, t) - probability(q, Elem<T>::to_f(qrow[at]), at, t);
-      if (w > 0.0) k = log(w) + gv;
-    } else {
-      k = (p.b == INFINITY ? 0.0 : (double)x / t) + gv;
-    }
-    sh.kept[atomicAdd(&sh.n, 1)] = Best{k, at, x};
+  const bool last = at >= 0 && key >= unordered(sh.bar) - kMargin;
+  Best mine{-INFINITY, -1, 0.f};
+  // Two of one thread's columns too close for fp32: all columns by their exact keys.
+  const bool again = __syncthreads_or(last && near);
+  for (int v = again ? lo + threadIdx.x : last ? at : hi; v < hi; v = again ? v + kDrawThreads : hi) {
+    const float x = clean(Elem<T>::to_f(row[v]));
+    bool out = x == -INFINITY || (p.b == INFINITY && x != INFINITY);
+    for (int j = 0; j < n_skip; ++j) out |= skip[j] == v;
+    const double k = out ? (double)NAN : exact(v, x);
+    if (k == k) mine = better(mine, Best{k, v, x});
   }
+  if (last && mine.at < 0) mine = Best{key * 0.6931471805599453, at, clean(Elem<T>::to_f(row[at]))};
+  if (mine.at >= 0) sh.kept[atomicAdd(&sh.n, 1)] = mine;
   __syncthreads();
   Best b{-INFINITY, -1, 0.f};
   if (warp == 0) {

@@ -732,6 +732,30 @@ def test_sample_accept_odd_logits(cuda_device):
     assert got[1][2].tolist() == [0, -1, -1] and float(got[2][2, 0]) == -math.inf
 
 
+@pytest.mark.parametrize("with_draft", [False, True])
+def test_sample_accept_neighbouring_columns_that_fp32_cannot_tell_apart(cuda_device, with_draft):
+    """Two neighbours whose keys differ by 1e-7 at a key of 40: the greater wins, wherever it lies; equal ones: the lower."""
+    B, V = 64, 4096
+    target = torch.full((B, 2, V), -5.0)
+    target[:, :, 7] = 30.0
+    draft = torch.full((B, 1, V), -5.0)
+    draft[:, :, 5] = 60.0
+    gumbel = torch.zeros(B, V)
+    drafts = torch.full((B, 1), 5, dtype=torch.int32)
+    want = []
+    for b in range(B):
+        c = 8 + 61 * b
+        gumbel[b, c:c + 2] = 60.0
+        target[b, :, c] = 0.0
+        target[b, :, c + 1] = (b % 3 - 1) * 1.2e-7  # below, the same, above
+        want.append(c + 1 if b % 3 == 2 else c)
+    u, t = torch.full((B, 1), 0.5), torch.ones(B)  # rejected: q(5) is 1, p(5) e^-35
+    got = ops.sample_accept(*[x.to(cuda_device) for x in (target, drafts, u, gumbel, t)],
+                            draft_logits=draft.to(cuda_device) if with_draft else None)
+    assert got[0].tolist() == [0] * B and got[1][:, 0].tolist() == want
+    assert plain_chain(target, drafts, u, gumbel, t, draft if with_draft else None)[1] == got[1].tolist()
+
+
 def test_sample_accept_draws_from_the_target(cuda_device):
     """Whatever the draft, the first emitted token is distributed as the target's: counts within five
     standard deviations (fixed seed), with a draft distribution, and with drafts that have none."""
