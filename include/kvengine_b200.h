@@ -434,7 +434,7 @@ int kve_kv_read_fp8(const void* pool_k, const void* pool_v, const uint8_t* k_sca
  * logits: [batch, k+1, vocab] rows row_stride elements apart (fp32 or bf16); draft_logits
  * (same dtype): row j of sequence b at b * stride_b + j * stride_j; drafts as for
  * kve_greedy_accept; uniforms [batch, k] rows uniform_stride_b apart; gumbel
- * [batch, vocab] fp32 rows gumbel_stride apart; temperature [batch] fp32. 1 <= k <= 31.
+ * [batch, vocab] fp32 rows gumbel_stride apart; temperature [batch] fp32. 1 <= k <= 31, vocab <= 2^30.
  * Outputs: n_accepted [batch], emitted [batch, k+1] (drafts[:n], the token drawn, -1), and
  * logprobs [batch, k+1]: log p of each emitted token (0 for T <= 0 and past the end). */
 size_t kve_sample_accept_workspace_bytes(int batch, int k, int vocab, int with_draft_logits);

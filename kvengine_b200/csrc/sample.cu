@@ -769,6 +769,7 @@ extern "C" int kve_sample_accept(const void* logits, int dtype, int64_t row_stri
       (draft_logits && (draft_logits_stride_b < 0 || draft_logits_stride_j < 0)))
     return set_error(KVE_ERR_ARG, "%s: bad sizes batch=%d k=%d vocab=%d", me, batch, k, vocab);
   if (dtype != KVE_F32 && dtype != KVE_BF16) return set_error(KVE_ERR_DTYPE, "%s: dtype %d", me, dtype);
+  if (vocab > (1 << 30)) return set_error(KVE_ERR_SHAPE, "%s: vocab %d > 2^30", me, vocab);
   if (batch == 0) return KVE_OK;
   if (!logits || !drafts || !uniforms || !gumbel || !temperature || !out_n_accepted || !out_emitted || !out_logprobs)
     return set_error(KVE_ERR_ARG, "%s: null pointer", me);
@@ -809,6 +810,7 @@ extern "C" int kve_tree_sample_accept(const void* logits, int dtype, int64_t row
     return set_error(KVE_ERR_ARG, "%s: bad sizes", me);
   if (max_q_len > kMaxNodes) return set_error(KVE_ERR_SHAPE, "%s: max_q_len %d > %d", me, max_q_len, kMaxNodes);
   if (dtype != KVE_F32 && dtype != KVE_BF16) return set_error(KVE_ERR_DTYPE, "%s: dtype %d", me, dtype);
+  if (vocab > (1 << 30)) return set_error(KVE_ERR_SHAPE, "%s: vocab %d > 2^30", me, vocab);
   if (batch == 0) return KVE_OK;
   if (n_rows < 1) return set_error(KVE_ERR_ARG, "%s: no rows for %d sequences", me, batch);
   if (!logits || !tokens || !parents || !q_lens || !q_offsets || !uniforms || !gumbel || !temperature || !out_n_accepted ||

@@ -847,6 +847,24 @@ def test_tree_sample_accept(cuda_device, dt, V, shapes):
         same_logprobs(got[3][b:b + 1], [want[3]])
 
 
+def test_tree_sample_accept_largest_tree(cuda_device):
+    """1024 nodes: a chain that is accepted to its end, and a random tree beside it."""
+    g, rng = torch.Generator().manual_seed(47), random.Random(47)
+    trees = [[i - 1 for i in range(1024)], [-1] + [rng.randint(0, i - 1) for i in range(1, 1024)]]
+    V = 1500
+    logits, tokens, u = tree_inputs(trees, V, torch.float32, g, rng)
+    u[:1024] = 0.0
+    gumbel = -torch.empty(2, V).exponential_(generator=g).log()
+    t = torch.tensor([0.9, 1.1])
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    got = ops.tree_sample_accept(logits.to(cuda_device), tokens.to(cuda_device), i32(trees[0] + trees[1]), i32([1024, 1024]),
+                                 i32([0, 1024, 2048]), 1024, u.to(cuda_device), gumbel.to(cuda_device), t.to(cuda_device))
+    want = [plain_tree(logits[o:o + 1024], tokens[o:o + 1024], trees[b], u[o:o + 1024], gumbel[b], t[b], 1024)
+            for b, o in ((0, 0), (1, 1024))]
+    assert got[0].tolist() == [w[0] for w in want] and got[0].tolist()[0] == 1023
+    assert got[1].tolist() == [w[1] for w in want] and got[2].tolist() == [w[2] for w in want]
+
+
 def test_tree_sample_accept_stars_chains_and_bad_nodes(cuda_device):
     g, rng = torch.Generator().manual_seed(2), random.Random(2)
     V, wide = 300, 1024

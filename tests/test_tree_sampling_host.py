@@ -91,6 +91,7 @@ TREE = dict(logits=P, dtype=0, stride=1000, tokens=P, parents=P, q_lens=P, q_off
     (dict(logits=None), -1, "null pointer"), (dict(t=None), -1, "null pointer"), (dict(ws=None), -6, "workspace needs"),
     (dict(ws_bytes=65536), -6, "workspace needs"), (dict(ws=P + 8), -1, "aligned"),
     (dict(batch=1 << 29), -2, "too many rows"),
+    (dict(vocab=(1 << 30) + 1, stride=1 << 31, gs=1 << 31), -2, "vocab 1073741825"),
 ])
 def test_sample_accept_refusals(change, code, words):
     refused(code, words, L.load().kve_sample_accept(*dict(CHAIN, **change).values()))
@@ -101,6 +102,7 @@ def test_sample_accept_refusals(change, code, words):
     (dict(rows=0), -1, "no rows"), (dict(max_q=1025), -2, "max_q_len 1025"), (dict(dtype=5), -3, "dtype 5"),
     (dict(parents=None), -1, "null pointer"), (dict(path=None), -1, "null pointer"),
     (dict(ws_bytes=65535), -6, "workspace needs"),
+    (dict(vocab=(1 << 30) + 1, stride=1 << 31, gs=1 << 31), -2, "vocab 1073741825"),
 ])
 def test_tree_sample_accept_refusals(change, code, words):
     refused(code, words, L.load().kve_tree_sample_accept(*dict(TREE, **change).values()))
