@@ -90,7 +90,10 @@ constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
 // its first access, read or write, to global memory that an earlier kernel may
 // write (it returns once the kernels before it in the stream have completed and
 // their writes are visible); only inputs declared constant, such as model
-// weights in kve_forward, are read before it. grid_dep_launch() follows it.
+// weights in kve_forward, are read before it. grid_dep_launch() follows it, and
+// in a kernel that allocates tensor memory it follows the allocation too: a
+// dependent may allocate before its own wait, and an allocation that waits for
+// the columns of a CTA that waits for this kernel would never end.
 // Both are no-ops for a plain launch.
 // The wait is an inline-asm memory barrier, which the compiler honours only for
 // memory it cannot prove private: a load through a `const T* __restrict__` kernel

@@ -251,7 +251,6 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   grid_dep_wait();
-  grid_dep_launch();
 
   const int bh = blockIdx.x, c = blockIdx.y, qtile = blockIdx.z;
   const int b = bh / p.nkv, h = bh % p.nkv;
@@ -310,6 +309,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   if (warp == 3) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    grid_dep_launch();  // not before: a dependent's CTA here may hold columns and wait for this one
   }
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q);
   auto head_row = [&](int r) {  // row r of the CTA in q and out
