@@ -427,7 +427,8 @@ int kve_kv_read_fp8(const void* pool_k, const void* pool_v, const uint8_t* k_sca
  * the token behind it is argmax_v(log w_v + gumbel[b, v]), lowest v among equals, with
  * w = max(p_n - q_n, 0), or p_k where all were accepted, or p_n where no w is positive.
  * Uniforms in [0, 1) and Gumbel noise -log(-log u) give tokens distributed as sampling
- * from the target alone. T <= 0 (or NaN): p and q are one-hot at their lowest argmax.
+ * from the target alone. T <= 0 (or NaN): p and q are one-hot at their lowest argmax; a
+ * subnormal T counts as 2^-126.
  * A NaN logit counts as minus infinity; a row without any probability accepts nothing
  * and gives token 0 with log-probability -inf. A draft outside [0, vocab) is rejected
  * and recorded as KVE_ERR_BOUNDS.

@@ -26,13 +26,16 @@
 // 16 bf16 nodes (350 MB) 75 us, one bf16 chain 13 us. The first kernel takes three quarters of
 // the large ones, at 83 % of HBM's throughput; one chain is two kernels' latencies.
 //
-// Precision: a row is held as (b, z), z = sum 2^(x c - b) with c = log2(e) / T and
-// b the largest x c as rounded, so that every x c - b is one fused operation
-// rounded relative to itself, whatever the logits' size. 2^x runs on ex2.approx (2^-22)
+// Precision: a row is held as (b, z), z = sum 2^((x - b) c) with c = log2(e) / T and b the
+// largest logit. The sums are taken relative to b c as rounded, so that every exponent is one
+// fused operation rounded relative to itself, and moved by what the rounding left. That holds while
+// the rest is small: past |b c| of 2^22 (half an ulp would be an exponent of 1/4, at 3e9 more than fp32's
+// whole range) a row's exponents are (x - b) c from 64-bit differences, more slowly. 2^x runs on ex2.approx (2^-22)
 // into fp32 sums of a part's few dozen values per thread, then pairwise.
 // Acceptance, log-probabilities and the candidates within fp32 rounding of a CTA's
 // best are recomputed in 64 bits. A NaN logit counts as minus infinity (never drawn);
 // rows with one are summed again, slowly.
+#include <float.h>
 #include <math.h>
 
 #include "kve_common.cuh"
@@ -40,7 +43,7 @@
 namespace kve {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 constexpr int kStatThreads = 256;
 constexpr int kDrawThreads = 256;  // and three CTAs a SM: 128 sequences' clusters run in one wave
 constexpr int kMaxParts = 32;     // parts of a row in the first kernel
@@ -54,6 +57,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The temperature as it counts: 0 where T <= 0 or NaN, and subnormal numbers as 2^-126 (c stays finite).
+__device__ __forceinline__ float heat(float t) { return t > 0.f ? fmaxf(t, FLT_MIN) : 0.f; }
 // NaN as minus infinity.
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
 
@@ -110,8 +115,8 @@ __device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch
   for (int j = head + nvec * N + threadIdx.x; j < hi; j += THREADS) one(Elem<T>::to_f(row[j]), j);
 }
 
-// What the first kernel leaves of one part of a row: its base and its sum, or, for
-// T <= 0, its largest logit and that one's column.
+// What the first kernel leaves of one part of a row: its largest logit, and the sum relative to
+// that or, for T <= 0, its column.
 struct Part {
   float b, z;
 };
@@ -146,6 +151,21 @@ __device__ __forceinline__ const T* row_at(const Rows& r, int row) {
   return static_cast<const T*>(r.second) + (i / r.k) * r.second_sb + (i % r.k) * r.second_sj;
 }
 
+// 1 / T to 2^-46: one fp32 quotient and its remainder, a fraction of a 64-bit division's latency.
+__device__ __forceinline__ double inverse(float t) {
+  if (t > 1e30f) return 1.0 / t;  // fp32's quotient would be subnormal
+  const float r = 1.f / t;
+  return (double)r + (double)r * fmaf(-t, r, 1.f);
+}
+// log2 of e^(x / T) over e^(b / T) in 64 bits, b a row's largest logit (an infinite one: only its likes count).
+__device__ __forceinline__ double exponent(float x, float b, float t) {
+  return b == INFINITY ? (x == INFINITY ? 0.0 : -INFINITY) : ((double)x - b) * (kLog2e * inverse(t));
+}
+
+// Whether fp32 exponents fused from x c will not do for a row of largest logit b: b c is too large (or
+// infinite), or c so small that a difference of logits may overflow and still count.
+__device__ __forceinline__ bool far(float b, float c) { return !(fabsf(b * c) < 4194304.f) || c < 1e-30f; }
+
 template <typename T>
 __global__ void __launch_bounds__(kStatThreads, 4)
 row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temperature, Part* out) {
@@ -153,7 +173,7 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
   grid_dep_launch();
   const int row = blockIdx.x, part = blockIdx.y;
   const int lo = part * chunk, hi = min(vocab, lo + chunk);
-  const float t = temperature[sequence_of(rows, row)];
+  const float t = heat(temperature[sequence_of(rows, row)]);
   const T* x = row_at<T>(rows, row);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ float sm[kStatThreads / 32], sz[kStatThreads / 32];
@@ -186,18 +206,18 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
     }
     return;
   }
-  const float c = kLog2e / t;
-  float base = -INFINITY, z = 0.f;  // this thread's b and z
+  const float c = (float)kLog2e / t;
+  float most = -INFINITY, off = 0.f, z = 0.f;  // this thread's largest logit, minus that times c, and the sum
   auto rebase = [&](float top) {
-    top *= c;
-    if (top > base) {
-      z *= ex2(base - top);  // 0 at the first
-      base = top;
+    if (top > most) {
+      z *= ex2(-off - top * c);  // of nothing at the first
+      most = top;
+      off = -(top * c);
     }
   };
   auto one = [&](float v, int) {
     rebase(v);
-    z += ex2(fmaf(v, c, base == -INFINITY ? 0.f : -base));
+    z += ex2(fmaf(v, c, off));
   };
   auto batch = [&](auto& v, int) {
     constexpr int N = Pack<T>::N;
@@ -205,7 +225,6 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
 #pragma unroll
     for (int j = 1; j < N; ++j) top = fmaxf(top, v[j]);  // passes over NaN
     rebase(top);
-    const float off = base == -INFINITY ? 0.f : -base;
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = ex2(fmaf(v[j], c, off));
 #pragma unroll
@@ -226,20 +245,20 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
     for (int o = kStatThreads / 64; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
   };
-  float top = block_max(base);
-  bool odd = __syncthreads_or(!(z < INFINITY));  // a NaN, or infinite logits
-  if (odd) {
+  const float top = block_max(most);
+  const bool odd = __syncthreads_or(!(z < INFINITY));  // a NaN, or infinite logits
+  if (top == -INFINITY) {
+    z = 0.f;
+  } else if (odd || far(top, c)) {
     // infinite logits share the whole probability, NaN has none
-    base = -INFINITY;
-    for (int i = lo + threadIdx.x; i < hi; i += kStatThreads) base = fmaxf(base, Elem<T>::to_f(x[i]) * c);
-    top = block_max(base);
     z = 0.f;
     for (int i = lo + threadIdx.x; i < hi; i += kStatThreads) {
       const float v = clean(Elem<T>::to_f(x[i]));
-      if (v != -INFINITY) z += top == INFINITY ? (v == INFINITY ? 1.f : 0.f) : ex2(fmaf(v, c, -top));
+      if (v != -INFINITY) z += ex2((float)exponent(v, top, t));
     }
   } else {
-    z = base == -INFINITY ? 0.f : z * ex2(base - top);
+    const float b = top * c;
+    z = most == -INFINITY ? 0.f : z * ex2(-off - b - fmaf(top, c, -b));
   }
   z = warp_sum(z);
   if (lane == 0) sz[warp] = z;
@@ -253,8 +272,8 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
 
 // A row's parts joined.
 struct Row {
-  double z;   // the sum of 2^(x c - b)
-  float b;    // the base (T <= 0: the largest logit)
+  double z;   // the sum of 2^((x - b) c)
+  float b;    // the largest logit
   int arg;    // T <= 0: the column of the largest
 };
 // Rows row_of(0) .. row_of(n - 1) into out, by all threads: `group` (a power of two of at
@@ -276,21 +295,22 @@ __device__ __forceinline__ void join_rows(const Part* parts, int n_parts, int gr
       r.arg = sub < n_parts && p.b == b ? __float_as_int(p.z) : 0x7fffffff;
       for (int o = 1; o < group; o <<= 1) r.arg = min(r.arg, __shfl_xor_sync(0xffffffffu, r.arg, o));
     } else {
-      r.z = p.b == -INFINITY ? 0.0 : p.b == b ? (double)p.z : (double)p.z * exp2((double)p.b - b);
+      r.z = p.b == -INFINITY ? 0.0 : p.b == b ? (double)p.z : (double)p.z * exp2(exponent(p.b, b, t));
       for (int o = 1; o < group; o <<= 1) r.z += __shfl_xor_sync(0xffffffffu, r.z, o);
     }
     if (i < n && sub == 0) out[i] = r;
   }
 }
-// log2 of e^(x / T) over e^(the base), and p of logit x at column v, in 64 bits.
-__device__ __forceinline__ double exponent(float x, float b, float t) {
-  return b == INFINITY ? (x == INFINITY ? 0.0 : -INFINITY) : (double)x * (double)(kLog2e / t) - b;
-}
+// p of logit x at column v in 64 bits, and its logarithm (T > 0).
 __device__ __forceinline__ double probability(const Row& r, float x, int v, float t) {
   if (!(t > 0.f)) return v == r.arg ? 1.0 : 0.0;
   x = clean(x);
   if (x == -INFINITY || !(r.z > 0.0)) return 0.0;
   return exp2(exponent(x, r.b, t)) / r.z;
+}
+__device__ __forceinline__ float log_probability(const Row& r, float x, float t) {
+  if (clean(x) == -INFINITY || !(r.z > 0.0)) return -INFINITY;
+  return (float)((log2(r.z) - exponent(x, r.b, t)) * -0.6931471805599453);
 }
 struct DrawParams {
   const void* logits;       // target rows
@@ -366,14 +386,20 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
                                              const Row& q, const float* gumbel, float t, const int* skip, int n_skip) {
   constexpr int N = Pack<T>::N;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr float kL = (float)kLog2e;
+  const float c = kL / t;
+  if (q.b == -INFINITY) qrow = nullptr;  // a draft without any probability takes nothing away
+  const bool slow = far(p.b, c) || (qrow && far(q.b, c));  // every column in 64 bits
   __syncthreads();  // an earlier draw's values have been read
   if (threadIdx.x == 0) {
     sh.bar = ordered(-INFINITY);
     sh.n = 0;
-    sh.lz = (float)log2(p.z);
-    sh.inv_zp = (float)(1.0 / p.z);
+    // the scan's exponents are relative to p.b c as rounded
+    const float moved = slow ? 0.f : fmaf(p.b, c, -(p.b * c));
+    sh.lz = (float)log2(p.z) + moved;
+    sh.inv_zp = (float)(1.0 / p.z) * ex2(-moved);
   } else if (threadIdx.x == 32) {
-    sh.inv_zq = qrow && q.z > 0.0 ? (float)(1.0 / q.z) : 0.f;
+    sh.inv_zq = qrow && !slow ? (float)(1.0 / q.z) * ex2(-fmaf(q.b, c, -(q.b * c))) : 0.f;
   }
   // 16 bytes of logits at a time from their first 16-byte boundary on, and their noise
   const int mis = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
@@ -401,15 +427,15 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
   int at = -1;
   bool near = false;  // this thread passed over a column whose key was within kMargin of its best one's
   __syncthreads();
-  if (p.z > 0.0) {
-    const float c = kLog2e / t, lz = sh.lz, off = p.b == INFINITY ? 0.f : -p.b;
-    auto weigh = [&](float x) { return p.b == INFINITY ? (x == INFINITY ? 0.f : -INFINITY) : fmaf(x, c, off); };
+  if (p.z > 0.0 && !slow) {
+    const float lz = sh.lz, off = -(p.b * c), qoff = -(q.b * c);
+    auto weigh = [&](float x) { return fmaf(x, c, off); };
     volatile int* bar = &sh.bar;
     auto consider = [&](float e, float gv, int v) {  // e: log2 of the weight without the draft, times z
       float k = e - lz + gv;
       if (qrow) {
         const float y = clean(Elem<T>::to_f(qrow[v]));
-        const float qw = q.b == INFINITY ? (y == INFINITY ? 1.f : 0.f) : ex2(fmaf(y, c, -q.b));
+        const float qw = ex2(fmaf(y, c, qoff));
         const float w = ex2(e) * sh.inv_zp - qw * sh.inv_zq;
         k = w > 0.f ? __log2f(w) + gv : -INFINITY;
       }
@@ -424,7 +450,7 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
       if (ordered(k) > *bar) atomicMax(&sh.bar, ordered(k));
     };
     auto one = [&](float x, int v) {
-      const float e = weigh(clean(x)), gv = gumbel[v] * kLog2e;
+      const float e = weigh(clean(x)), gv = gumbel[v] * kL;
       if (e - lz + gv > unordered(*bar) - kMargin) consider(e, gv, v);
     };
     auto batch = [&](const float* x, const float* g, int v) {
@@ -433,12 +459,12 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         e[j] = weigh(x[j]);
-        top = fmaxf(top, fmaf(g[j], kLog2e, e[j]));
+        top = fmaxf(top, fmaf(g[j], kL, e[j]));
       }
       if (!(top - lz > unordered(*bar) - kMargin)) return;
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (fmaf(g[j], kLog2e, e[j]) - lz > unordered(*bar) - kMargin) consider(e[j], g[j] * kLog2e, v + j);
+        if (fmaf(g[j], kL, e[j]) - lz > unordered(*bar) - kMargin) consider(e[j], g[j] * kL, v + j);
     };
     for (int i = lo + threadIdx.x; i < head; i += kDrawThreads) one(Elem<T>::to_f(row[i]), i);
     constexpr int U = sizeof(T) == 4 ? 4 : 2;
@@ -463,15 +489,15 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
   }
   // Column v's key in 64 bits; NaN where its weight rounds to nothing there.
   auto exact = [&](int v, float x) {
-    if (!qrow) return (p.b == INFINITY ? 0.0 : (double)x / t) + (double)gumbel[v];
+    if (!qrow) return (p.b == INFINITY ? 0.0 : ((double)x - p.b) * inverse(t)) + (double)gumbel[v];
     const double w = probability(p, x, v, t) - probability(q, Elem<T>::to_f(qrow[v]), v, t);
     return w > 0.0 ? log(w) + (double)gumbel[v] : (double)NAN;
   };
   __syncthreads();
   const bool last = at >= 0 && key >= unordered(sh.bar) - kMargin;
   Best mine{-INFINITY, -1, 0.f};
-  // Two of one thread's columns too close for fp32: all columns by their exact keys.
-  const bool again = __syncthreads_or(last && near);
+  // Two of one thread's columns too close for fp32, or a row that fp32 does not do for: all columns by their exact keys.
+  const bool again = __syncthreads_or(last && near) || (p.z > 0.0 && slow);
   for (int v = again ? lo + threadIdx.x : last ? at : hi; v < hi; v = again ? v + kDrawThreads : hi) {
     const float x = clean(Elem<T>::to_f(row[v]));
     bool out = x == -INFINITY || (p.b == INFINITY && x != INFINITY);
@@ -535,7 +561,7 @@ chain_draw_kernel(DrawParams a) {
   grid_dep_launch();
   const int b = blockIdx.x / a.shares, rank = blockIdx.x % a.shares;
   const int k = a.k, tid = threadIdx.x;
-  const float t = a.temperature[b];
+  const float t = heat(a.temperature[b]);
   const T* logits = static_cast<const T*>(a.logits) + (int64_t)b * (k + 1) * a.stride;
   const T* draft = a.draft ? static_cast<const T*>(a.draft) + b * a.dsb : nullptr;
   __shared__ Row rows[2 * kMaxK + 1];  // target rows 0 .. k, then draft rows
@@ -586,7 +612,7 @@ chain_draw_kernel(DrawParams a) {
   }
   if (rank != 0 || tid > k) return;
   float lp = 0.f;
-  if (t > 0.f && tid <= n) lp = (float)log(tid < n ? pd[tid] : probability(p, last.x, last.at, t));
+  if (t > 0.f && tid <= n) lp = tid < n ? (float)log(pd[tid]) : log_probability(p, last.x, t);
   a.emitted[(size_t)b * a.width + tid] = tid < n ? tok[tid] : tid == n ? last.at : -1;
   a.logp[(size_t)b * a.width + tid] = lp;
   if (tid == 0) a.n_acc[b] = n;
@@ -607,7 +633,7 @@ tree_draw_kernel(DrawParams a) {
   const int b = blockIdx.x / a.shares, rank = blockIdx.x % a.shares;
   const int tid = threadIdx.x;
   const int n = a.q_lens[b], off = a.q_offsets[b];
-  const float t = a.temperature[b];
+  const float t = heat(a.temperature[b]);
   // every CTA of the cluster sees the same values: all leave or none
   if (n < 1 || n > a.max_nodes || off < 0 || off > a.n_rows - n) {
     if (tid == 0 && rank == 0) {
@@ -689,7 +715,7 @@ tree_draw_kernel(DrawParams a) {
     const int child = j < m ? path[j + 1] : -1;
     a.path[to] = j <= m ? path[j] : -1;
     a.emitted[to] = j < m ? tok[child] : j == m ? last.at : -1;
-    a.logp[to] = t > 0.f && j <= m ? (float)log(j < m ? pt[child] : probability(p, last.x, last.at, t)) : 0.f;
+    a.logp[to] = !(t > 0.f) || j > m ? 0.f : j < m ? (float)log(pt[child]) : log_probability(p, last.x, t);
   }
   if (tid == 0) a.n_acc[b] = m;
 }
