@@ -32,8 +32,8 @@
 // the rest is small: past |b c| of 2^22 (half an ulp would be an exponent of 1/4, at 3e9 more than fp32's
 // whole range) a row's exponents are (x - b) c from 64-bit differences, more slowly. 2^x runs on ex2.approx (2^-22)
 // into fp32 sums of a part's few dozen values per thread, then pairwise.
-// Acceptance, log-probabilities and the candidates within fp32 rounding of a CTA's
-// best are recomputed in 64 bits. A NaN logit counts as minus infinity (never drawn);
+// Acceptance, log-probabilities and every candidate that fp32 does not rule out are computed in 64
+// bits from these sums. A NaN logit counts as minus infinity (never drawn);
 // rows with one are summed again, slowly.
 #include <float.h>
 #include <math.h>
@@ -361,8 +361,8 @@ struct DrawShared {
   Best kept[kDrawThreads];
   Best share[8];               // rank 0's: the best of each CTA of the cluster
   Best best;
-  float lz, inv_zp, inv_zq;    // log2 z of the target's row; 1 / z of it and of the draft's
-  int bar;                     // the CTA's best fp32 key so far, as an ordered integer
+  float ratio;                 // z of the target's row over that of the draft's
+  int bar;                     // what a column has to reach to be the CTA's best, as an ordered integer
   int n;                       // candidates kept
 };
 __device__ __forceinline__ int ordered(float f) {
@@ -371,16 +371,19 @@ __device__ __forceinline__ int ordered(float f) {
 }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i < 0 ? i ^ 0x7fffffff : i); }
 
-// Keys (log2 of a weight, plus gumbel log2 e) in fp32 are good to a few 1e-6; what lies
-// this close below the best is looked at in 64 bits.
-constexpr float kMargin = 1e-4f;
+// What fp32 may be off by, relative to the size of each term of a key or weight: exponents, ex2.approx and
+// lg2.approx are good to 2^-22, and a handful of roundings of 2^-24 come on top.
+constexpr float kOff = 0x1p-20f;
 
 // The CTA's best candidate of columns [lo, hi), in every lane of warp 0. `qrow` (may be
 // null): the draft's row, whose distribution is subtracted. `skip`: tokens not to draw.
 //
-// A column's key is at most its key without the draft, so the scan compares that
-// with the CTA's best so far, and only the few columns that pass it cost an
-// exponential, a logarithm and a look at the draft's row.
+// A column's key is log2 of its weight plus gumbel log2 e. The scan in fp32 knows it only to
+// lie between two bounds; where p and q nearly cancel they are far apart. It keeps the largest
+// lower bound of the CTA's columns, and every column whose upper bound reaches that is looked at in 64 bits, so the
+// result is that of 64 bits (from the rows' sums as they are). A key is at most the one without the
+// draft, so a column is first held against that, and only the few that pass cost an exponential, a
+// logarithm and a look at the draft's row.
 template <typename T>
 __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, const T* row, const Row& p, const T* qrow,
                                              const Row& q, const float* gumbel, float t, const int* skip, int n_skip) {
@@ -392,14 +395,10 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
   const bool slow = far(p.b, c) || (qrow && far(q.b, c));  // every column in 64 bits
   __syncthreads();  // an earlier draw's values have been read
   if (threadIdx.x == 0) {
-    sh.bar = ordered(-INFINITY);
+    sh.bar = ordered(-FLT_MAX);  // which minus infinity does not reach
     sh.n = 0;
-    // the scan's exponents are relative to p.b c as rounded
-    const float moved = slow ? 0.f : fmaf(p.b, c, -(p.b * c));
-    sh.lz = (float)log2(p.z) + moved;
-    sh.inv_zp = (float)(1.0 / p.z) * ex2(-moved);
-  } else if (threadIdx.x == 32) {
-    sh.inv_zq = qrow && !slow ? (float)(1.0 / q.z) * ex2(-fmaf(q.b, c, -(q.b * c))) : 0.f;
+    // z of p over z of q, for sums relative to b c as rounded
+    if (qrow && !slow) sh.ratio = (float)(p.z / q.z) * ex2(fmaf(p.b, c, -(p.b * c)) - fmaf(q.b, c, -(q.b * c)));
   }
   // 16 bytes of logits at a time from their first 16-byte boundary on, and their noise
   const int mis = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
@@ -423,48 +422,63 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
       for (int j = 0; j < N; ++j) g[j] = gh[(size_t)i * N + j];
     }
   };
-  float key = -INFINITY;
-  int at = -1;
-  bool near = false;  // this thread passed over a column whose key was within kMargin of its best one's
+  int at = -1;                                                 // this thread's column of the largest lower bound,
+  float low = -INFINITY, high = -INFINITY, other = -INFINITY;  // its bounds, and the others' largest upper bound
   __syncthreads();
   if (p.z > 0.0 && !slow) {
-    const float lz = sh.lz, off = -(p.b * c), qoff = -(q.b * c);
-    auto weigh = [&](float x) { return fmaf(x, c, off); };
+    // Keys times z here. Exponents are fused from x c and relative to b c as rounded;
+    const float off = -(p.b * c), qoff = -(q.b * c);
     volatile int* bar = &sh.bar;
-    auto consider = [&](float e, float gv, int v) {  // e: log2 of the weight without the draft, times z
-      float k = e - lz + gv;
+    // Upper bounds without the draft are u = e + g (1 + 8 kOff). A key k = e + g, e at most 0, is at most
+    // u + 10 kOff |k| + 4 kOff: positive noise brings along more than e can be off by, and with negative noise
+    // neither term is larger than k. So a column with u below bar - 16 kOff (|bar| + 1) is below the bar, and that is what sh.bar holds.
+    constexpr float kMore = kL * (1.f + 8.f * kOff);
+    auto consider = [&](float x, float g, float u, int v) {
+      if (!(x > -INFINITY)) return;
+      const float gl = g * kL, e = fmaf(x, c, off), sure = fabsf(gl) < INFINITY ? kOff : 0.f;  // infinite noise: nothing is off
+      float least = u - (sure > 0.f ? 16.f * sure * (fabsf(e) + fabsf(gl) + 1.f) : 0.f);
       if (qrow) {
-        const float y = clean(Elem<T>::to_f(qrow[v]));
-        const float qw = ex2(fmaf(y, c, qoff));
-        const float w = ex2(e) * sh.inv_zp - qw * sh.inv_zq;
-        k = w > 0.f ? __log2f(w) + gv : -INFINITY;
+        const float y = clean(Elem<T>::to_f(qrow[v])), f = fmaf(y, c, qoff);
+        const float pw = ex2(e), qw = ex2(f) * sh.ratio;  // times z
+        // below 2^-110 a weight is only known to be small
+        const float off_by = kOff * (pw * (2.f + fminf(fabsf(e), 200.f)) + qw * (4.f + fminf(fabsf(f), 200.f))) + 0x1p-110f;
+        const float hi_w = pw - qw + off_by, lo_w = pw - qw - off_by;
+        auto key = [&](float w, float way) {
+          const float l = __log2f(w);
+          return l + gl + (sure > 0.f ? way * sure * (fabsf(l) + fabsf(gl) + 2.f) : 0.f);
+        };
+        u = hi_w > 0.f ? fminf(u, key(hi_w, 1.f)) : -INFINITY;
+        least = lo_w > 0.f ? key(lo_w, -1.f) : -INFINITY;
+        if (!(u >= unordered(*bar))) return;
       }
-      if (!(k > key - kMargin)) return;
       for (int j = 0; j < n_skip; ++j)
         if (skip[j] == v) return;
-      near = k < key + kMargin;
-      if (k > key) {
-        key = k;
+      if (at < 0 || least > low) {
+        other = fmaxf(other, high);
         at = v;
+        low = least;
+        high = u;
+      } else {
+        other = fmaxf(other, u);
       }
-      if (ordered(k) > *bar) atomicMax(&sh.bar, ordered(k));
+      const int b = ordered(fabsf(least) < INFINITY ? least - 16.f * kOff * (fabsf(least) + 1.f) : least);
+      if (b > *bar) atomicMax(&sh.bar, b);
     };
     auto one = [&](float x, int v) {
-      const float e = weigh(clean(x)), gv = gumbel[v] * kL;
-      if (e - lz + gv > unordered(*bar) - kMargin) consider(e, gv, v);
+      const float g = gumbel[v], u = fmaf(g, kMore, fmaf(x, c, off));
+      if (u >= unordered(*bar)) consider(x, g, u, v);
     };
     auto batch = [&](const float* x, const float* g, int v) {
-      float top = -INFINITY;
-      float e[N];
+      float u[N], top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        e[j] = weigh(x[j]);
-        top = fmaxf(top, fmaf(g[j], kL, e[j]));
+        u[j] = fmaf(g[j], kMore, fmaf(x[j], c, off));
+        top = fmaxf(top, u[j]);  // passes over NaN
       }
-      if (!(top - lz > unordered(*bar) - kMargin)) return;
+      if (!(top >= unordered(*bar))) return;
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (fmaf(g[j], kL, e[j]) - lz > unordered(*bar) - kMargin) consider(e[j], g[j] * kL, v + j);
+        if (u[j] >= unordered(*bar)) consider(x[j], g[j], u[j], v + j);
     };
     for (int i = lo + threadIdx.x; i < head; i += kDrawThreads) one(Elem<T>::to_f(row[i]), i);
     constexpr int U = sizeof(T) == 4 ? 4 : 2;
@@ -494,10 +508,11 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
     return w > 0.0 ? log(w) + (double)gumbel[v] : (double)NAN;
   };
   __syncthreads();
-  const bool last = at >= 0 && key >= unordered(sh.bar) - kMargin;
+  const float bar = unordered(sh.bar);
+  const bool last = at >= 0 && high >= bar;
   Best mine{-INFINITY, -1, 0.f};
-  // Two of one thread's columns too close for fp32, or a row that fp32 does not do for: all columns by their exact keys.
-  const bool again = __syncthreads_or(last && near) || (p.z > 0.0 && slow);
+  // Another of one thread's columns that may be the best, or a row that fp32 does not do for: all columns.
+  const bool again = __syncthreads_or(other >= bar) || (p.z > 0.0 && slow);
   for (int v = again ? lo + threadIdx.x : last ? at : hi; v < hi; v = again ? v + kDrawThreads : hi) {
     const float x = clean(Elem<T>::to_f(row[v]));
     bool out = x == -INFINITY || (p.b == INFINITY && x != INFINITY);
@@ -505,7 +520,6 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
     const double k = out ? (double)NAN : exact(v, x);
     if (k == k) mine = better(mine, Best{k, v, x});
   }
-  if (last && mine.at < 0) mine = Best{key * 0.6931471805599453, at, clean(Elem<T>::to_f(row[at]))};
   if (mine.at >= 0) sh.kept[atomicAdd(&sh.n, 1)] = mine;
   __syncthreads();
   Best b{-INFINITY, -1, 0.f};

@@ -1,4 +1,5 @@
-"""Sampling, draft trees and the 8-bit cache at their limits: temperatures and logits of every size.
+"""Sampling, draft trees and the 8-bit cache at their limits: temperatures and logits of every size,
+drafts whose distribution is nearly the target's.
 
 Tolerances as in test_gpu_tree_sampling.py, which derives them.
 """
@@ -97,3 +98,53 @@ def test_sampling_at_an_infinite_temperature(cuda_device):
     want = torch.where(live, gumbel, -math.inf).argmax(-1)
     assert n.tolist() == [0] * B and emitted[:, 0].tolist() == want.tolist()
     assert bool(((logp[:, 0].cpu() + math.log(int(live.sum()))).abs() <= 1e-5).all())
+
+
+# ---------------------------------------------------------------- drafts whose distribution is nearly the target's
+def near_chain(B, V, g, eps, bump):
+    """One draft a sequence, its logits eps away from the target's, its own raised by `bump`: it is rejected."""
+    target = torch.randn(B, 2, V, generator=g) * 2
+    draft = (target[:, :1] + eps * torch.randn(B, 1, V, generator=g)).float()
+    p = target[:, 0].double().softmax(-1)
+    drafts = (p - 1e-5).abs().argmin(-1)  # a token of about 1e-5: little of the residual is its doing
+    draft[torch.arange(B), 0, drafts] += bump
+    return target, draft, drafts[:, None].int(), torch.full((B, 1), 0.9999), gumbels(B, V, g=g), torch.ones(B)
+
+
+@pytest.mark.parametrize("V", [2000, 32000])
+@pytest.mark.parametrize("bump", [0.2, 1.0, 3.0])
+def test_residual_of_equal_distributions_but_for_one_token(cuda_device, V, bump):
+    """p - q is a small share of p, the same for every other token (their logits are equal): the draw is that from
+    p without the draft, whatever the share. p and q are good to 2^-20 together, the share here is above
+    1e-5 (e^bump - 1): its sign is certain, and the order is that of log p + gumbel, which 64 bits tell apart."""
+    g = torch.Generator().manual_seed(V)
+    target, draft, drafts, u, gumbel, t = near_chain(400, V, g, 0.0, bump)
+    got = ops.sample_accept(*[x.to(cuda_device) for x in (target, drafts, u, gumbel, t)], draft_logits=draft.to(cuda_device))
+    key = target[:, 0].double() + gumbel.double()
+    key.scatter_(1, drafts.long(), -math.inf)
+    assert got[0].tolist() == [0] * 400 and got[1][:, 0].tolist() == key.argmax(-1).tolist()
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("eps", [1e-2, 1e-3, 1e-4, 1e-5, 1e-6])
+def test_residual_of_nearly_equal_distributions(cuda_device, dt, eps):
+    """The token drawn is the argmax of log(p - q) + gumbel for some p and q within their error: with both off
+    by at most r of themselves (2^-21 for the exponentials and sums, the exponents' 2^-22 times their
+    mean size under p), its greatest key reaches every other token's least."""
+    g = torch.Generator().manual_seed(11)
+    B, V = 400, 32000
+    target, draft, drafts, u, gumbel, t = near_chain(B, V, g, eps, 2.0)
+    target, draft = target.to(dt), draft.to(dt)
+    n, emitted, _ = ops.sample_accept(*[x.to(cuda_device) for x in (target, drafts, u, gumbel, t)],
+                                      draft_logits=draft.to(cuda_device))
+    p, q = target[:, 0].double().softmax(-1), draft[:, 0].double().softmax(-1)
+    rejected = 0.9999 * q.gather(1, drafts.long()) >= p.gather(1, drafts.long())
+    assert bool(rejected.all()) and n.tolist() == [0] * B
+    top = target[:, 0].double()
+    r = 2.0 ** -21 + 2.0 ** -22 * 1.4427 * float((p * (top.amax(-1, keepdim=True) - top)).sum(-1).max())
+    greatest = ((p - q) + r * (p + q)).clamp(min=0).log() + gumbel.double()
+    least = ((p - q) - r * (p + q)).clamp(min=0).log() + gumbel.double()
+    assert bool((least.amax(-1) > -math.inf).all())
+    bar = least.amax(-1)
+    chosen = greatest.gather(1, emitted[:, :1].long().cpu())[:, 0]
+    assert bool((chosen >= bar).all()), int((chosen < bar).sum())
