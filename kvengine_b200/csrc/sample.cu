@@ -31,7 +31,8 @@
 // fused operation rounded relative to itself, and moved by what the rounding left. That holds while
 // the rest is small: past |b c| of 2^22 (half an ulp would be an exponent of 1/4, at 3e9 more than fp32's
 // whole range) a row's exponents are (x - b) c from 64-bit differences, more slowly. 2^x runs on ex2.approx (2^-22)
-// into fp32 sums of a part's few dozen values per thread, then pairwise.
+// into fp32 sums of up to 128 of a thread's vectors, those into a 64-bit one, and the threads' pairwise in
+// fp32 again: p is good to about 2^-21 and 2^-22 times the mean size of the exponents (c's rounding).
 // Acceptance, log-probabilities and every candidate that fp32 does not rule out are computed in 64
 // bits from these sums. A NaN logit counts as minus infinity (never drawn);
 // rows with one are summed again, slowly.
@@ -85,9 +86,10 @@ template <> struct Pack<__nv_bfloat16> {
 };
 
 // Calls f(value, index) for columns [lo, hi) of a row, 16 bytes at a time from the
-// row's first 16-byte boundary on; `batch(values, first index, n)` gets the vectors.
-template <typename T, int THREADS, int U, typename Batch, typename One>
-__device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch, One&& one) {
+// row's first 16-byte boundary on; `batch(values, first index)` gets the vectors, and `fold()` is
+// called now and then in a long row, after every 16 U of a thread's vectors.
+template <typename T, int THREADS, int U, typename Batch, typename One, typename Fold>
+__device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch, One&& one, Fold&& fold) {
   constexpr int N = Pack<T>::N;
   const int off = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
   const int head = min(lo + (off ? N - off : 0), hi);
@@ -95,7 +97,7 @@ __device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch
   const uint4* v = reinterpret_cast<const uint4*>(row + head);
   for (int i = lo + threadIdx.x; i < head; i += THREADS) one(Elem<T>::to_f(row[i]), i);
   int i = threadIdx.x;
-  for (; i + (U - 1) * THREADS < nvec; i += U * THREADS) {
+  for (int rest = 16; i + (U - 1) * THREADS < nvec; i += U * THREADS) {
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = __ldcg(v + i + u * THREADS);
@@ -104,6 +106,10 @@ __device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch
       float x[N];
       Pack<T>::unpack(raw[u], x);
       batch(x, head + (i + u * THREADS) * N);
+    }
+    if (--rest == 0) {
+      fold();
+      rest = 16;
     }
   }
   for (; i < nvec; i += THREADS) {
@@ -129,7 +135,7 @@ struct Rows {
   int64_t first_stride;             // elements between consecutive rows
   int64_t second_sb, second_sj;     // elements between sequences, and between a sequence's rows
   int n_first, per_seq, k;          // target rows, and rows of a sequence in each of the two (chain)
-  const int32_t* q_offsets;         // tree: a row's sequence is found here (batch + 1 entries)
+  const int32_t* q_offsets;         // tree: a row's sequence is found here (batch entries)
   int batch;
 };
 
@@ -188,7 +194,7 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
 #pragma unroll
       for (int j = 0; j < Pack<T>::N; ++j) one(v[j], i + j);
     };
-    scan<T, kStatThreads, 2>(x, lo, hi, batch, one);
+    scan<T, kStatThreads, 2>(x, lo, hi, batch, one, [] {});
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float ov = __shfl_xor_sync(0xffffffffu, best, o);
@@ -207,7 +213,9 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
     return;
   }
   const float c = (float)kLog2e / t;
-  float most = -INFINITY, off = 0.f, z = 0.f;  // this thread's largest logit, minus that times c, and the sum
+  float most = -INFINITY, off = 0.f, z = 0.f;  // this thread's largest logit, minus that times c, and its latest terms' sum
+  double sum = 0.0;                            // the others' (a long row's terms are below half an ulp of an fp32 sum),
+  float sum_off = 0.f;                         // relative to this
   auto rebase = [&](float top) {
     if (top > most) {
       z *= ex2(-off - top * c);  // of nothing at the first
@@ -233,7 +241,12 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
       for (int j = 0; j < w; ++j) v[j] += v[j + w];
     z += v[0];
   };
-  scan<T, kStatThreads, 8>(x, lo, hi, batch, one);
+  auto fold = [&] {
+    sum = sum == 0.0 ? z : sum * ex2(off - sum_off) + z;
+    sum_off = off;
+    z = 0.f;
+  };
+  scan<T, kStatThreads, 8>(x, lo, hi, batch, one, fold);
   // the part's base, then its sum
   auto block_max = [&](float v) {
 #pragma unroll
@@ -246,20 +259,22 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
     return v;
   };
   const float top = block_max(most);
-  const bool odd = __syncthreads_or(!(z < INFINITY));  // a NaN, or infinite logits
+  fold();
+  const bool odd = __syncthreads_or(!(sum < INFINITY));  // a NaN, or infinite logits
   if (top == -INFINITY) {
-    z = 0.f;
+    sum = 0.0;
   } else if (odd || far(top, c)) {
     // infinite logits share the whole probability, NaN has none
-    z = 0.f;
+    sum = 0.0;
     for (int i = lo + threadIdx.x; i < hi; i += kStatThreads) {
       const float v = clean(Elem<T>::to_f(x[i]));
-      if (v != -INFINITY) z += ex2((float)exponent(v, top, t));
+      if (v != -INFINITY) sum += ex2((float)exponent(v, top, t));
     }
   } else {
     const float b = top * c;
-    z = most == -INFINITY ? 0.f : z * ex2(-off - b - fmaf(top, c, -b));
+    sum = most == -INFINITY ? 0.0 : sum * ex2(-off - b - fmaf(top, c, -b));
   }
+  z = (float)sum;
   z = warp_sum(z);
   if (lane == 0) sz[warp] = z;
   __syncthreads();

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from kvengine_b200 import ops
-from test_gpu_tree_sampling import plain_chain, plain_tree, same_logprobs
+from test_gpu_tree_sampling import U32, plain_chain, plain_tree, same_logprobs
 
 pytestmark = pytest.mark.gpu
 
@@ -98,6 +98,23 @@ def test_sampling_at_an_infinite_temperature(cuda_device):
     want = torch.where(live, gumbel, -math.inf).argmax(-1)
     assert n.tolist() == [0] * B and emitted[:, 0].tolist() == want.tolist()
     assert bool(((logp[:, 0].cpu() + math.log(int(live.sum()))).abs() <= 1e-5).all())
+
+
+@pytest.mark.parametrize("dt, V", [(torch.bfloat16, (1 << 28) + 3), (torch.float32, (1 << 27) + 1), (torch.bfloat16, (1 << 30))])
+def test_sample_accept_over_long_rows(cuda_device, dt, V):
+    """Sums of 2^30 terms, each below half an ulp of what a thread has summed: the log-probability is that of the
+    count. And tokens beyond 2^29 are drawn by their keys."""
+    x = torch.full((1, 2, V), -0.357, dtype=dt, device=cuda_device)
+    x[:, :, ::1021] = 0.0  # some in every thread's share
+    gumbel = torch.zeros(1, V, device=cuda_device)
+    gumbel[0, V - 2] = 3.0
+    n, emitted, logp = ops.sample_accept(x, torch.full((1, 1), 7, dtype=torch.int32, device=cuda_device),
+                                         torch.full((1, 1), 0.999, device=cuda_device), gumbel,
+                                         torch.ones(1, device=cuda_device))
+    e, tops = float(x[0, 0, 1]), -(-V // 1021)
+    want = float(x[0, 0, V - 2]) - math.log(tops + (V - tops) * math.exp(e))
+    assert n.tolist() == [0] and emitted[:, 0].tolist() == [V - 2]
+    assert abs(float(logp[0, 0]) - want) <= 2.0 ** -22 + 3 * U32 + 64 * U32 + U32 * abs(want)
 
 
 # ---------------------------------------------------------------- drafts whose distribution is nearly the target's
