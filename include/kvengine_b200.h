@@ -448,7 +448,8 @@ int kve_sample_accept(const void* logits, int dtype, int64_t row_stride, const v
 
 /* Verification of trees of candidate tokens by sampling. Sequence b's tree has q_lens[b]
  * nodes, rows q_offsets[b] .. of logits [n_rows, vocab], tokens, parents and uniforms
- * [n_rows]; q_offsets [batch] ascends. Node 0 is the token before the tree (its
+ * [n_rows]; q_offsets [batch] ascends, that of a sequence without nodes too, and
+ * sequences share no rows. Node 0 is the token before the tree (its
  * logits predict its children; its token, parent and uniform are not read); the
  * others have 0 <= parent < their own index. From node 0: the children of the
  * current node in index order, child c with token d accepted (and then current)
@@ -458,8 +459,9 @@ int kve_sample_accept(const void* logits, int dtype, int64_t row_stride, const v
  * where those have no probability). p, T, NaN and the noise as for kve_sample_accept.
  * A node with a token or parent out of range is nobody's child and recorded as
  * KVE_ERR_BOUNDS. max_q_len <= 1024.
- * Outputs: n_accepted [batch] (-1 for a sequence without nodes, whose other outputs
- * are not written), and, [batch, max_q_len]: path (the accepted nodes, node 0 first, then
+ * Outputs: n_accepted [batch] (-1 for a sequence without nodes, and, recorded as
+ * KVE_ERR_BOUNDS, for one whose length or rows do not fit or, by offsets that do not ascend, got
+ * another sequence's temperature; its other outputs are not written), and, [batch, max_q_len]: path (the accepted nodes, node 0 first, then
  * -1), emitted (their tokens without node 0's, the token drawn, then -1), logprobs. */
 size_t kve_tree_sample_accept_workspace_bytes(int n_rows, int vocab);
 int kve_tree_sample_accept(const void* logits, int dtype, int64_t row_stride, const int32_t* tokens,

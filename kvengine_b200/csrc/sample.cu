@@ -139,15 +139,19 @@ struct Rows {
   int batch;
 };
 
-__device__ __forceinline__ int sequence_of(const Rows& r, int row) {
-  if (!r.q_offsets) return row < r.n_first ? row / r.per_seq : (row - r.n_first) / r.k;
-  int lo = 0, hi = r.batch;  // the last b with q_offsets[b] <= row
+// The last b with offsets[b] <= row, where they ascend; in any case no less for a greater row.
+__device__ __forceinline__ int search(const int32_t* offsets, int batch, int row) {
+  int lo = 0, hi = batch;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (r.q_offsets[mid] <= row) lo = mid;
+    if (offsets[mid] <= row) lo = mid;
     else hi = mid;
   }
   return lo;
+}
+__device__ __forceinline__ int sequence_of(const Rows& r, int row) {
+  if (r.q_offsets) return search(r.q_offsets, r.batch, row);
+  return row < r.n_first ? row / r.per_seq : (row - r.n_first) / r.k;
 }
 
 template <typename T>
@@ -680,10 +684,17 @@ tree_draw_kernel(DrawParams a) {
   int* next = reinterpret_cast<int*>(us + a.max_nodes);
   int* path = next + a.max_nodes;
   int* skip = path + a.max_nodes;
-  __shared__ int s_n, s_skip;
+  __shared__ int s_n, s_skip, s_strange;
   __shared__ DrawShared sh;
   const T* logits = static_cast<const T*>(a.logits) + (int64_t)off * a.stride;
   if (tid == 0) s_skip = 0;
+  // Where offsets do not ascend or sequences share rows, the sums may be of another sequence's temperature: they
+  // are this one's if the first and the last row (then also those between) are found to be of one sequence with it.
+  if (tid >= kDrawThreads - 32) {
+    const int found = search(a.q_offsets, a.batch, tid == kDrawThreads - 1 ? off + n - 1 : off);
+    const int last = __shfl_sync(0xffffffffu, found, 31);
+    if (tid == kDrawThreads - 32) s_strange = found != last || heat(a.temperature[found]) != t;
+  }
   for (int i = tid; i < n; i += kDrawThreads) {
     int d = a.drafts[off + i], pa = a.parents[off + i];
     us[i] = a.u[off + i];
@@ -699,6 +710,14 @@ tree_draw_kernel(DrawParams a) {
   }
   join_rows(a.parts, a.n_parts, a.group, t, rows, n, [&](int i) { return off + i; });
   __syncthreads();
+  if (s_strange) {
+    if (tid == 0 && rank == 0) {
+      report(a.status, KVE_ERR_BOUNDS);
+      a.n_acc[b] = -1;
+    }
+    cluster_wait();
+    return;
+  }
   // p of every node's token at its parent: 0 for a token an earlier sibling has too
   for (int i = tid; i < n; i += kDrawThreads) {
     const int pa = par[i];

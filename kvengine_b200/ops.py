@@ -527,8 +527,10 @@ def tree_sample_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torc
                        status: torch.Tensor | None = None, out=None):
     """Verification of draft trees by sampling (kve_tree_sample_accept): logits [N, V] and tokens,
     parents (int32), uniforms [N] of the trees' nodes, sequence b's at rows q_offsets[b] .. +
-    q_lens[b] (parents within the tree, node 0 its root); gumbel [B, V], temperature [B] ->
-    (n_accepted [B], path, emitted, logprobs [B, max_q_len]). `out` may give the four."""
+    q_lens[b] (parents within the tree, node 0 its root; offsets ascend, rows are not shared); gumbel
+    [B, V], temperature [B] -> (n_accepted [B], path, emitted, logprobs [B, max_q_len]). A sequence
+    without nodes gets n_accepted -1, and its rows of the other three are not written. `out` may
+    give the four."""
     if out is None:
         r = L.fast().tree_sample_accept(logits, tokens, parents, q_lens, q_offsets, max_q_len, uniforms, gumbel,
                                         temperature, None if workspace is None else workspace.buf, status)

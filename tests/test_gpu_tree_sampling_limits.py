@@ -117,6 +117,42 @@ def test_sample_accept_over_long_rows(cuda_device, dt, V):
     assert abs(float(logp[0, 0]) - want) <= 2.0 ** -22 + 3 * U32 + 64 * U32 + U32 * abs(want)
 
 
+def test_tree_sample_accept_refuses_rows_of_another_temperature(cuda_device):
+    """Offsets that do not ascend, or rows that two sequences share, would give a row the sums of another
+    sequence's temperature: such a sequence is reported and left out, the others are right, and where the
+    temperatures are the same nothing is wrong."""
+    g = torch.Generator().manual_seed(2)
+    V, n, tree = 700, 5, [-1, 0, 0, 1, 1]
+    logits = torch.randn(3 * n, V, generator=g) * 3
+    tokens = torch.randint(0, V, (3 * n,), generator=g, dtype=torch.int32)
+    for b in range(3):
+        tokens[b * n + 1] = int(logits[b * n].argmax())
+    u, gumbel = torch.rand(3 * n, generator=g) * 0.5, gumbels(4, V, g=g)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    for offsets, lens, temps, good in (
+            ([0, 5, 10, 15], [5, 5, 5, 0], [0.7, 0.0, 1.3, 0.4], [0, 1, 2]),   # as documented, one without nodes
+            ([0, 5, 10, 0], [5, 5, 5, 0], [0.7, 0.0, 1.3, 0.4], None),         # the padding's offset does not ascend
+            ([10, 0, 5, 15], [5, 5, 5, 0], [0.7, 0.0, 1.3, 0.4], None),
+            ([0, 0, 5, 10], [5, 5, 5, 5], [0.7, 0.9, 1.3, 0.4], [1, 2, 3]),    # shared rows, of two temperatures
+            ([0, 0, 5, 10], [5, 5, 5, 5], [0.7, 0.7, 0.0, 0.4], [0, 1, 2, 3]),  # of one
+            ([0, 3, 5, 10], [5, 5, 5, 5], [0.7, 0.9, 1.3, 0.4], [2, 3])):
+        status = ops.status_tensor(cuda_device)
+        t = torch.tensor(temps)
+        got = ops.tree_sample_accept(logits.to(cuda_device), tokens.to(cuda_device), i32(tree * 3), i32(lens), i32(offsets), n,
+                                     u.to(cuda_device), gumbel.to(cuda_device), t.to(cuda_device), status=status)
+        live = [b for b in range(4) if lens[b]]
+        right = []
+        for b in live:
+            s = slice(offsets[b], offsets[b] + n)
+            want = plain_tree(logits[s], tokens[s], tree, u[s], gumbel[b], t[b], n)
+            if int(got[0][b]) != -1:
+                assert (int(got[0][b]), got[1][b].tolist(), got[2][b].tolist()) == want[:3], (offsets, b)
+                same_logprobs(got[3][b:b + 1], [want[3]])
+                right.append(b)
+        assert good is None or right == good, (offsets, right)
+        assert (int(status) == -7) == (right != live), offsets
+
+
 # ---------------------------------------------------------------- drafts whose distribution is nearly the target's
 def near_chain(B, V, g, eps, bump):
     """One draft a sequence, its logits eps away from the target's, its own raised by `bump`: it is rejected."""
