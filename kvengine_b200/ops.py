@@ -274,6 +274,21 @@ def _call(fn, index: int, *args) -> None:
         L.check(rc)
 
 
+def _status(name: str, index: int, status) -> int | None:
+    if status is None:
+        return None
+    _dense(name, index, (status, _I32))
+    if status.numel() < 1:
+        _refuse(name, "status must have an element")
+    return status.data_ptr()
+
+
+def _space(name: str, index: int, workspace, device, need: int) -> torch.Tensor:
+    buf = (workspace or Workspace(device)).get(need)
+    _dense(name, index, (buf, _U8))  # a workspace of another device would be written there
+    return buf
+
+
 def _fp8_cache(name: str, index: int, k, v, k_scale, v_scale) -> None:
     _dense(name, index, (k, _E4M3), (v, _E4M3), (k_scale, _U8), (v_scale, _U8))
     shape = k.shape
@@ -351,11 +366,12 @@ def tree_attention(q, pool_k_layer, pool_v_layer, block_tables, ctx_lens, q_lens
     need = _tree_attn_ws(B, max_q_len, max_ctx, nq, nkv, hd)
     ws, ws_bytes = None, 0
     if need:
-        buf = (workspace or Workspace(q.device)).get(need)
+        buf = _space("tree_attention", dev, workspace, q.device, need)
         ws, ws_bytes = buf.data_ptr(), buf.numel()
     _call(lib.kve_paged_tree_attn, dev, q.data_ptr(), code, pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), kv_code, ks, vs,
           block_tables.data_ptr(), width, ctx_lens.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(), mask, words, B, n,
-          max_q_len, max_ctx, nq, nkv, hd, bs, num_blocks, scale, out.data_ptr(), ws, ws_bytes, L.ptr(status))
+          max_q_len, max_ctx, nq, nkv, hd, bs, num_blocks, scale, out.data_ptr(), ws, ws_bytes,
+          _status("tree_attention", dev, status))
     return out
 
 
@@ -405,7 +421,7 @@ def qkv_rope_append_fp8(qkv, positions, slots, rope_cos, rope_sin, q_out, pool_k
     _call(lib.kve_qkv_rope_append_fp8, dev, qkv.data_ptr(), L.dtype_code(dtype), n, num_heads, num_kv_heads, head_dim,
           positions.data_ptr(), slots.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), rope_len, q_out.data_ptr(),
           pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks * bs,
-          L.ptr(status))
+          _status(name, dev, status))
 
 
 def kv_append_fp8(k_new, v_new, slot_ids, pool_k_layer, pool_v_layer, k_scale, v_scale, status=None) -> None:
@@ -421,7 +437,7 @@ def kv_append_fp8(k_new, v_new, slot_ids, pool_k_layer, pool_v_layer, k_scale, v
                                  f"{list(pool_k_layer.shape)}")
     _call(lib.kve_kv_append_fp8, dev, k_new.data_ptr(), v_new.data_ptr(), L.dtype_code(dtype), slot_ids.data_ptr(), n, nkv,
           hd, pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_blocks * bs,
-          L.ptr(status))
+          _status("kv_append_fp8", dev, status))
 
 
 def kv_read_fp8(pool_k_layer, pool_v_layer, k_scale, v_scale, slot_ids, dtype: torch.dtype = torch.bfloat16, out=None,
@@ -449,7 +465,8 @@ def kv_read_fp8(pool_k_layer, pool_v_layer, k_scale, v_scale, slot_ids, dtype: t
         if k.shape != (n, nkv, hd) or v.shape != (n, nkv, hd):
             _refuse("kv_read_fp8", f"out must be two tensors [{n}, {nkv}, {hd}]")
     _call(lib.kve_kv_read_fp8, dev, pool_k_layer.data_ptr(), pool_v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-          slot_ids.data_ptr(), n, nkv, hd, num_blocks * bs, L.dtype_code(dtype), k.data_ptr(), v.data_ptr(), L.ptr(status))
+          slot_ids.data_ptr(), n, nkv, hd, num_blocks * bs, L.dtype_code(dtype), k.data_ptr(), v.data_ptr(),
+          _status("kv_read_fp8", dev, status))
     return k, v
 
 
@@ -513,11 +530,11 @@ def sample_accept(logits: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Te
         _dense(name, dev, (n_acc, _I32), (emitted, _I32), (logprobs, _F32))
         if n_acc.numel() != B or emitted.shape != (B, kp1) or logprobs.shape != (B, kp1):
             _refuse(name, f"out must be [{B}], [{B}, {kp1}] and [{B}, {kp1}]")
-    ws = (workspace or Workspace(logits.device)).get(_sample_ws(B, k, V, int(dl is not None)))
+    ws = _space(name, dev, workspace, logits.device, _sample_ws(B, k, V, int(dl is not None)))
     dsb, dsj = drafts.stride()
     _call(lib.kve_sample_accept, dev, logits.data_ptr(), L.dtype_code(dtype), stride, dl, dlb, dlj, drafts.data_ptr(), dsb,
           dsj, uniforms.data_ptr(), usb, gumbel.data_ptr(), gs, temperature.data_ptr(), B, k, V, n_acc.data_ptr(),
-          emitted.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), ws.numel(), L.ptr(status))
+          emitted.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), ws.numel(), _status(name, dev, status))
     return n_acc, emitted, logprobs
 
 
@@ -562,11 +579,11 @@ def tree_sample_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torc
         shape = (B, max_q_len)
         if n_acc.numel() != B or path.shape != shape or emitted.shape != shape or logprobs.shape != shape:
             _refuse(name, f"out must be [{B}] and three times [{B}, {max_q_len}]")
-    ws = (workspace or Workspace(logits.device)).get(_tree_sample_ws(N, V))
+    ws = _space(name, dev, workspace, logits.device, _tree_sample_ws(N, V))
     _call(lib.kve_tree_sample_accept, dev, logits.data_ptr(), L.dtype_code(dtype), stride, tokens.data_ptr(),
           parents.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(), uniforms.data_ptr(), gumbel.data_ptr(), gs,
           temperature.data_ptr(), B, N, max_q_len, V, n_acc.data_ptr(), path.data_ptr(), emitted.data_ptr(),
-          logprobs.data_ptr(), ws.data_ptr(), ws.numel(), L.ptr(status))
+          logprobs.data_ptr(), ws.data_ptr(), ws.numel(), _status(name, dev, status))
     return n_acc, path, emitted, logprobs
 
 
@@ -602,4 +619,4 @@ def kv_commit_path(pool_k, pool_v, block_tables, start_lens, path, n_accepted, k
         _refuse("kv_commit_path", "one block table row, path row, start and count per sequence")
     _call(lib.kve_kv_commit_path, dev, pool_k.data_ptr(), pool_v.data_ptr(), code, ks, vs, layers, num_blocks, bs, nkv, hd,
           block_tables.data_ptr(), width, start_lens.data_ptr(), path.data_ptr(), path_width, n_accepted.data_ptr(), B,
-          L.ptr(status))
+          _status("kv_commit_path", dev, status))
