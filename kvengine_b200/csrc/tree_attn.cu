@@ -314,12 +314,17 @@ tree_attn_kernel(TreeParams p) {
         else report(p.status, KVE_ERR_BOUNDS);  // reads as zeros
       }
       if constexpr (KV == kFp8) {
-        // the aligned word that holds the key's scale byte (lanes 16.. : V's), and the byte's place
+        // the aligned word that holds the key's scale byte (lanes 16.. : V's) up to that byte, and the byte's
+        // place; where the scales begin inside that word, the byte alone
         if (rb == 0) {
-          const uint8_t* s = (lane < 16 ? p.k_scale : p.v_scale) + (slot < 0 ? 0 : slot * p.nkv + h);
-          const uint32_t at = (uint32_t)(reinterpret_cast<uintptr_t>(s) & 3u);
-          cp4(sring + st * 256 + lane * 4, s - at, slot < 0 ? 0u : 4u);
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(sring + st * 256 + 128 + lane * 4), "r"(at * 8) : "memory");
+          const uint8_t* all = lane < 16 ? p.k_scale : p.v_scale;
+          const uint8_t* s = all + (slot < 0 ? 0 : slot * p.nkv + h);
+          const uint32_t at = (uint32_t)(reinterpret_cast<uintptr_t>(s) & 3u), to = sring + st * 256 + lane * 4;
+          if (slot >= 0 && (size_t)(s - all) < at)
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"((uint32_t)*s << at * 8) : "memory");
+          else
+            cp4(to, s - at, slot < 0 ? 0u : at + 1);
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + 128), "r"(at * 8) : "memory");
         }
       }
       constexpr int PIECES = 2 * kTile * CH;  // K then V

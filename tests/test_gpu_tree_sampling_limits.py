@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from kvengine_b200 import ops
-from test_gpu_tree_sampling import U32, plain_chain, plain_tree, same_logprobs
+from test_gpu_tree_sampling import U32, attention_case, check_attention, plain_chain, plain_tree, same_logprobs
 
 pytestmark = pytest.mark.gpu
 
@@ -201,3 +201,22 @@ def test_residual_of_nearly_equal_distributions(cuda_device, dt, eps):
     bar = least.amax(-1)
     chosen = greatest.gather(1, emitted[:, :1].long().cpu())[:, 0]
     assert bool((chosen >= bar).all()), int((chosen < bar).sum())
+
+
+# ---------------------------------------------------------------- the 8-bit cache's scales
+@pytest.mark.parametrize("heads, nodes, bs", [((3, 3, 64), [2, 1], 1), ((4, 1, 128), [2, 1], 7), ((3, 3, 64), [5, 9], 1),
+                                              ((6, 1, 128), [9, 4], 7), ((6, 3, 64), [1, 2], 16)])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+def test_scales_that_start_and_end_anywhere(cuda_device, heads, nodes, bs, shift):
+    """Scales that are a slice of a larger buffer, at any byte, and end inside an aligned word."""
+    args, *lens = attention_case("fp8", heads, nodes, [37, 90], bs, "tree", 12, cuda_device)
+    want = ops.tree_attention(**args)
+    check_attention(args, *lens, want)
+    for name in ("k_scale", "v_scale"):
+        n = args[name].numel()
+        buf = torch.full((n + 8,), 255, dtype=torch.uint8, device=cuda_device)
+        args[name] = buf[shift:shift + n].view(args[name].shape).copy_(args[name])
+    status = ops.status_tensor(cuda_device)
+    got = ops.tree_attention(**args, status=status)
+    check_attention(args, *lens, got)
+    assert int(status) == 0
