@@ -374,7 +374,7 @@ int kve_spec_next_draft_plan(const int32_t* start_lens, const int32_t* last_toke
  * attends all of the history and the nodes t whose bit is set in its mask words:
  * bit t % 32 of tree_mask[(q_offsets[b] + node) * mask_words + t / 32], t < q_lens[b]
  * (a node's own bit is not implied; mask_words >= ceil(max_q_len / 32)). tree_mask
- * NULL: nodes up to itself (a chain). A row that sees no key gets zeros; K and V
+ * NULL: nodes up to itself (a chain). A row that sees no key, or only keys whose scores are minus infinity, gets zeros; K and V
  * of nodes that a row does not see do not reach it, infinities and NaN included.
  * dtype: of q and out (KVE_BF16 or KVE_F32); kv_dtype: the same, or KVE_FP8_E4M3 for
  * bf16 queries over a cache written by the *_fp8 ops, with the layer's scale bytes

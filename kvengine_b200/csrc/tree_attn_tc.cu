@@ -745,6 +745,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     if (my_steps > 0) ok = ok && mbar_wait(smem_u32(&o_ready[grp]), 0, p.status);
     tc_after();
+    if (m == -INFINITY) l = 0.f;  // no score but minus infinity: ex2_fma's 2^-126 are no weights
   }
   // Every role is done; a wait that ran out anywhere leaves the outputs unwritten.
   const bool failed = __syncthreads_or(!ok);

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from kvengine_b200 import ops
-from test_gpu_tree_sampling import U32, attention_case, check_attention, plain_chain, plain_tree, same_logprobs
+from test_gpu_tree_sampling import U16, U32, attention_case, check_attention, plain_chain, plain_tree, same_logprobs, values
 
 pytestmark = pytest.mark.gpu
 
@@ -220,3 +220,66 @@ def test_scales_that_start_and_end_anywhere(cuda_device, heads, nodes, bs, shift
     got = ops.tree_attention(**args, status=status)
     check_attention(args, *lens, got)
     assert int(status) == 0
+
+
+# ---------------------------------------------------------------- infinities in the history
+def exact_rows(args, ctx, nodes, off):
+    """The formula in 64 bits, a score of minus infinity being a weight of 0 (a row of nothing else: zeros), and the
+    bound on the error of the outputs: that of test_gpu_tree_sampling.py over the keys with finite scores."""
+    q, mask = args["q"].cpu().double(), args["tree_mask"].cpu()
+    k, v = values(args["pool_k_layer"].cpu(), None if args["k_scale"] is None else args["k_scale"].cpu()), \
+        values(args["pool_v_layer"].cpu(), None if args["v_scale"] is None else args["v_scale"].cpu())
+    bs, nkv, hd = k.shape[1:]
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    for b, (c, n, o) in enumerate(zip(ctx, nodes, off)):
+        t, pos = args["block_tables"][b].cpu().long(), torch.arange(c)
+        kk, vv = k[t[pos // bs], pos % bs], v[t[pos // bs], pos % bs]
+        bits = torch.tensor([[bool(int(mask[o + i, j // 32]) >> j % 32 & 1) for j in range(n)] for i in range(n)])
+        seen = torch.cat([torch.ones(n, c - n, dtype=torch.bool), bits], 1)
+        for h in range(q.shape[1]):
+            kh, vh, qh = kk[:, h // (q.shape[1] // nkv)], vv[:, h // (q.shape[1] // nkv)], q[o:o + n, h]
+            s = (qh[:, None] * kh[None]).sum(-1) * args["scale"]
+            live = seen & (s > -math.inf)
+            s = torch.where(live, s, -math.inf)
+            top = s.amax(-1, keepdim=True)
+            w = torch.where(live, (s - torch.where(top == -math.inf, 0.0, top)).exp(), 0.0)
+            w = w / w.sum(-1, keepdim=True).clamp(min=1e-300)
+            terms = torch.where(live[..., None], w[..., None] * vh[None], 0.0)
+            r, a = terms.sum(1), terms.abs().sum(1)
+            size = torch.where(live, (qh.abs()[:, None] * kh.abs()[None]).sum(-1), 0.0).amax(-1)[:, None] * args["scale"]
+            d = (hd + 4) * U32 * size + 2.0 ** -21
+            if args["q"].dtype == torch.float32:
+                e = 2 * (d + 2.0 ** -21 * size) * a + (2.0 ** -21 + c * U32) * a + U32 * r.abs()
+            else:
+                e = 2 * d * a + (U16 + 2.0 ** -14) * a + U16 * r.abs()
+            out[o:o + n, h], tol[o:o + n, h] = r, e * 1.01 + 1e-30
+    return out, tol
+
+
+def compare(got, want, tol):
+    got, fin = got.cpu().double(), torch.isfinite(want)
+    assert torch.equal(got[~fin].nan_to_num(7e300), want[~fin].nan_to_num(7e300))
+    assert bool(((got - want).abs() <= tol)[fin].all()), float(((got - want).abs() / tol)[fin].max())
+
+
+SHAPES = [((8, 2, 64), [1, 2]), ((8, 2, 64), [9, 4]), ((16, 2, 128), [40, 3])]
+
+
+@pytest.mark.parametrize("heads, nodes", SHAPES)
+@pytest.mark.parametrize("cache, share, nodes_seen", [("bf16", 0.5, False), ("bf16", 0.5, True), ("bf16", 1.0, False),
+                                                      ("bf16", 1.0, True), ("fp8", 1.0, False)])
+def test_scores_of_minus_infinity_in_the_history(cuda_device, cache, heads, nodes, share, nodes_seen):
+    """A key whose score is minus infinity has no weight; a row with no other key gets zeros. In e4m3, which has no
+    infinity, it is q that makes the scores infinite, all of them."""
+    args, ctx, nodes, off = attention_case(cache, heads, nodes, [700, 130], 16, "tree", 3, cuda_device)
+    if not nodes_seen:
+        args["tree_mask"].zero_()
+    k = args["pool_k_layer"]
+    if cache == "fp8":
+        k.view(torch.uint8)[..., 0] = 0x38  # 1
+        args["q"][..., 0] = -math.inf
+    else:
+        spare = torch.rand(k.shape[:-1], generator=torch.Generator().manual_seed(1)).to(cuda_device) >= share
+        k[..., 0] = torch.where(spare, 1.0, -math.inf)
+        args["q"][..., 0] = 1.0
+    compare(ops.tree_attention(**args), *exact_rows(args, ctx, nodes, off))
