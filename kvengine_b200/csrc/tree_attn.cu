@@ -31,7 +31,8 @@
 //         2^e multiplies the scores. P V runs in bf16, which has fp32's range:
 //         p 2^e is rounded as p would be, whatever the spread of the exponents.
 //   fp32  m16n8k8 on tf32 with both operands split in two, x = hi + lo, and
-//         hi hi + hi lo + lo hi summed: the terms left out are 2^-22 of the product.
+//         hi hi + hi lo + lo hi summed: the terms left out are 2^-22 of the product. Rows with
+//         infinities among their operands are computed again, key by key.
 // Scores, maxima, sums and outputs are fp32 throughout.
 //
 // Measured: fp32, 14 / 2 heads of 64, one tree of 9 nodes behind 131 keys, 9.1 us (27 us before row
@@ -677,6 +678,7 @@ tree_attn_kernel(TreeParams p) {
   // Partials of one (sequence x kv head, query tile): [chunk][row][HD + 4] (m and l behind the dims).
   constexpr int PROW = HD + 4;
   float* part0 = p.partials + ((size_t)bh * p.n_qtiles + qtile) * p.n_chunks * (RB * 16) * PROW;
+  bool nan = false;
   for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
     const int r = i / (HD / 4), d = i % (HD / 4) * 4;
     float m = -INFINITY;
@@ -695,6 +697,10 @@ tree_attn_kernel(TreeParams p) {
       o.z += x.z * w;
       o.w += x.w * w;
     }
+    if constexpr (KV == kF32) {
+      const float sum = o.x + o.y + o.z + o.w + l;
+      nan |= !(fabsf(sum) < INFINITY);
+    }
     if (live == 1) {
       store4(r, d, o, l);
     } else {
@@ -703,6 +709,10 @@ tree_attn_kernel(TreeParams p) {
       if (d == 0) *reinterpret_cast<float2*>(pr + HD) = make_float2(m, l);
     }
   }
+  // An infinity or a number next to the largest has no two halves (infinity minus infinity): rows that
+  // came out as not finite are computed again without them.
+  if (KV == kF32 && __syncthreads_or(nan))
+    attend_by_key<QT, false, HD, kThreads>(p, b, h, qoff, hist, key_lo, key_hi, row0, rows, warp, lane, live > 1, part0 + (size_t)c * (RB * 16) * PROW);
   if (live == 1) return;
 
   // The last of the tile's chunks to arrive joins them, in chunk order.

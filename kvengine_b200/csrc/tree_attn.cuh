@@ -1,6 +1,9 @@
-// What the two kernels of tree attention share: the parameters of a call, the
-// workspace's layout and the mask words.
+// What the kernels of tree attention share: the parameters of a call, the workspace's
+// layout, the mask words and the way round the products.
 #pragma once
+
+#include <cuda_fp8.h>
+#include <math.h>
 
 #include "kve_common.cuh"
 
@@ -76,6 +79,62 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* row, int words, in
 __device__ __forceinline__ uint32_t chain_bits(int node, int j0) {
   const int d = node - j0;
   return d < 0 ? 0u : d >= 31 ? ~0u : (2u << d) - 1u;
+}
+
+// Rows row0 .. row0 + rows - 1 of sequence b and kv head h over the keys [key_lo, key_hi), key by key over
+// what each row sees, in plain fp32: for the few calls in which the products of whole tiles give what the
+// formula does not, infinities among them. A warp a row, HD / 32 dims a lane. Into `out`, or, where
+// the keys are split, as [row][HD + 4] partials with m and l behind the dims into `part`. Q: of q, out and, but for FP8, the cache.
+template <typename Q, bool FP8, int HD, int THREADS>
+__device__ __forceinline__ void attend_by_key(const TreeParams& p, int b, int h, int qoff, int hist, int key_lo, int key_hi, int row0,
+                                              int rows, int warp, int lane, bool split, float* part) {
+  constexpr int DPL = HD / 32;
+  const int32_t* table = p.tables + (size_t)b * p.table_stride;
+  auto element = [](const void* pool, const uint8_t* scales, size_t row, int d) {
+    if constexpr (FP8)
+      return scale_value(scales[row]) * __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(pool)[row * HD + d], __NV_E4M3)));
+    else
+      return Elem<Q>::to_f(static_cast<const Q*>(pool)[row * HD + d]);
+  };
+  const float sl = p.scale * 1.4426950408889634f;
+  for (int r = warp; r < rows; r += THREADS / 32) {
+    const int gr = row0 + r, node = node_of(p, gr);
+    const size_t head = ((size_t)(qoff + node) * p.nq + h * p.group + gr - node * p.group) * HD;  // the row in q and out
+    const uint32_t* mask = p.mask ? p.mask + (size_t)(qoff + node) * p.mask_words : nullptr;
+    float qv[DPL], acc[DPL] = {};
+#pragma unroll
+    for (int d = 0; d < DPL; ++d) qv[d] = Elem<Q>::to_f(static_cast<const Q*>(p.q)[head + lane + 32 * d]);
+    float rm = -INFINITY, rl = 0.f;
+    for (int key = key_lo; key < key_hi; ++key) {
+      const int j = key - hist;
+      if (j >= 0 && !(mask ? mask_bits<1>(mask, p.mask_words, j) & 1u : j <= node)) continue;
+      const int blk = table[key / p.bs];
+      const bool in = blk >= 0 && blk < p.num_blocks;  // reported by the loader
+      const size_t at = in ? ((size_t)blk * p.bs + key % p.bs) * p.nkv + h : 0;
+      float s = 0.f;
+#pragma unroll
+      for (int d = 0; d < DPL; ++d) s += in ? qv[d] * element(p.pool_k, p.k_scale, at, lane + 32 * d) : 0.f;
+      s = warp_sum(s) * sl;
+      if (s > rm) {
+        const float f = ex2(rm - s);
+        rm = s;
+        rl *= f;
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) acc[d] *= f;
+      }
+      const float e = s == -INFINITY ? 0.f : ex2(s - rm);
+      rl += e;
+#pragma unroll
+      for (int d = 0; d < DPL; ++d)
+        if (e != 0.f) acc[d] += in ? e * element(p.pool_v, p.v_scale, at, lane + 32 * d) : 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < DPL; ++d) {
+      if (!split) static_cast<Q*>(p.out)[head + lane + 32 * d] = Elem<Q>::from_f(rl == 0.f ? 0.f : acc[d] / rl);
+      else part[(size_t)r * (HD + 4) + lane + 32 * d] = acc[d];
+    }
+    if (split && lane == 0) *reinterpret_cast<float2*>(part + (size_t)r * (HD + 4) + HD) = make_float2(rm, rl);
+  }
 }
 
 }  // namespace kve

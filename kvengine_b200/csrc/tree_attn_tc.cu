@@ -840,54 +840,7 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
   }
   if (!failed && recompute) {
-    // Key by key over what each row sees: a warp a row, HD / 32 dims a lane.
-    constexpr int DPL = HD / 32;
-    const int32_t* table = p.tables + (size_t)b * p.table_stride;
-    auto element = [&](const void* pool, const uint8_t* scales, size_t row, int d) {
-      if constexpr (FP8) {
-        return scale_value(scales[row]) * __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(pool)[row * HD + d], __NV_E4M3)));
-      } else {
-        return __bfloat162float(static_cast<const __nv_bfloat16*>(pool)[row * HD + d]);
-      }
-    };
-    const float sl = p.scale * 1.4426950408889634f;
-    for (int r = warp; r < rows; r += threads_of(FP8) / 32) {
-      const int node = node_of(p, row0 + r);
-      const uint32_t* mask = p.mask ? p.mask + (size_t)(qoff + node) * p.mask_words : nullptr;
-      float qv[DPL], acc[DPL] = {};
-#pragma unroll
-      for (int d = 0; d < DPL; ++d) qv[d] = __bfloat162float(q[head_row(r) + lane + 32 * d]);
-      float rm = -INFINITY, rl = 0.f;
-      for (int key = key_lo; key < key_hi; ++key) {
-        const int j = key - hist;
-        if (j >= 0 && !(mask ? mask_bits<1>(mask, p.mask_words, j) & 1u : j <= node)) continue;
-        const int blk = table[key / p.bs];
-        const bool in = blk >= 0 && blk < p.num_blocks;  // reported by the loader
-        const size_t at = in ? ((size_t)blk * p.bs + key % p.bs) * p.nkv + h : 0;
-        float s = 0.f;
-#pragma unroll
-        for (int d = 0; d < DPL; ++d) s += in ? qv[d] * element(p.pool_k, p.k_scale, at, lane + 32 * d) : 0.f;
-        s = warp_sum(s) * sl;
-        if (s > rm) {
-          const float f = ex2(rm - s);
-          rm = s;
-          rl *= f;
-#pragma unroll
-          for (int d = 0; d < DPL; ++d) acc[d] *= f;
-        }
-        const float e = s == -INFINITY ? 0.f : ex2(s - rm);
-        rl += e;
-#pragma unroll
-        for (int d = 0; d < DPL; ++d)
-          if (e != 0.f) acc[d] += in ? e * element(p.pool_v, p.v_scale, at, lane + 32 * d) : 0.f;
-      }
-#pragma unroll
-      for (int d = 0; d < DPL; ++d) {
-        if (live == 1) out[head_row(r) + lane + 32 * d] = __float2bfloat16_rn(rl == 0.f ? 0.f : acc[d] / rl);
-        else part[(size_t)r * PROW + lane + 32 * d] = acc[d];
-      }
-      if (live > 1 && lane == 0) *reinterpret_cast<float2*>(part + (size_t)r * PROW + HD) = make_float2(rm, rl);
-    }
+    attend_by_key<__nv_bfloat16, FP8, HD, threads_of(FP8)>(p, b, h, qoff, hist, key_lo, key_hi, row0, rows, warp, lane, live > 1, part);
   }
   tc_before();
   __threadfence();

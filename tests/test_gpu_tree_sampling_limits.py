@@ -267,7 +267,8 @@ SHAPES = [((8, 2, 64), [1, 2]), ((8, 2, 64), [9, 4]), ((16, 2, 128), [40, 3])]
 
 @pytest.mark.parametrize("heads, nodes", SHAPES)
 @pytest.mark.parametrize("cache, share, nodes_seen", [("bf16", 0.5, False), ("bf16", 0.5, True), ("bf16", 1.0, False),
-                                                      ("bf16", 1.0, True), ("fp8", 1.0, False)])
+                                                      ("bf16", 1.0, True), ("fp8", 1.0, False), ("fp32", 0.5, False),
+                                                      ("fp32", 0.5, True), ("fp32", 1.0, False), ("fp32", 1.0, True)])
 def test_scores_of_minus_infinity_in_the_history(cuda_device, cache, heads, nodes, share, nodes_seen):
     """A key whose score is minus infinity has no weight; a row with no other key gets zeros. In e4m3, which has no
     infinity, it is q that makes the scores infinite, all of them."""
@@ -283,3 +284,27 @@ def test_scores_of_minus_infinity_in_the_history(cuda_device, cache, heads, node
         k[..., 0] = torch.where(spare, 1.0, -math.inf)
         args["q"][..., 0] = 1.0
     compare(ops.tree_attention(**args), *exact_rows(args, ctx, nodes, off))
+
+
+@pytest.mark.parametrize("heads, nodes", SHAPES)
+@pytest.mark.parametrize("cache", ["bf16", "fp32"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_infinite_values_in_the_history(cuda_device, cache, heads, nodes, value):
+    """Infinite elements of the history's V make their dims infinite in every row, opposite ones NaN, and leave
+    the others right."""
+    args, ctx, nodes, off = attention_case(cache, heads, nodes, [700, 130], 16, "tree", 6, cuda_device)
+    v, table = args["pool_v_layer"], args["block_tables"].tolist()
+    for b, pos, h, d in ((0, 0, 0, 5), (0, 399, 1, 17), (0, 650, 1, 63), (1, 64, 0, 0), (1, 100, 0, 1)):
+        v[table[b][pos // 16], pos % 16, h, d] = value
+    v[table[1][5], 3, 0, 0] = math.inf   # sequence 1, kv head 0, dim 0: infinity of either sign, or a NaN
+    compare(ops.tree_attention(**args), *exact_rows(args, ctx, nodes, off))
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (2, 2, 128)])
+def test_fp32_values_next_to_the_largest(cuda_device, heads):
+    """One key: its V comes back as it is, the largest numbers too."""
+    args, ctx, nodes, off = attention_case("fp32", heads, [1, 1], [0, 0], 16, "tree", 6, cuda_device)
+    args["pool_v_layer"][..., ::3] = torch.finfo(torch.float32).max
+    args["pool_v_layer"][..., 1::3] = -3.4e38
+    want, tol = exact_rows(args, ctx, nodes, off)
+    compare(ops.tree_attention(**args), want, tol)
