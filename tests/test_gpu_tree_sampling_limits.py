@@ -308,3 +308,75 @@ def test_fp32_values_next_to_the_largest(cuda_device, heads):
     args["pool_v_layer"][..., 1::3] = -3.4e38
     want, tol = exact_rows(args, ctx, nodes, off)
     compare(ops.tree_attention(**args), want, tol)
+
+
+# ---------------------------------------------------------------- the largest calls
+def check_on_device(args, ctx, nodes, off, got):
+    """check_attention for many rows: the same formula and bound, in 64 bits on the device."""
+    q, mask = args["q"].double(), args["tree_mask"]
+    k, v = values(args["pool_k_layer"], args["k_scale"]), values(args["pool_v_layer"], args["v_scale"])
+    bs, nkv, hd = k.shape[1:]
+    group = q.shape[1] // nkv
+    for b, (c, n, o) in enumerate(zip(ctx, nodes, off)):
+        pos = torch.arange(c, device=q.device)
+        t = args["block_tables"][b].long()
+        kk, vv = k[t[pos // bs], pos % bs], v[t[pos // bs], pos % bs]
+        j = torch.arange(n, device=q.device)
+        if mask is None:
+            bits = j[None] <= j[:, None]
+        else:
+            bits = (mask[o:o + n][:, j // 32] >> (j % 32)[None] & 1).bool()
+        seen = torch.cat([torch.ones(n, c - n, dtype=torch.bool, device=q.device), bits], 1)
+        for h in range(q.shape[1]):
+            qh, kh, vh = q[o:o + n, h], kk[:, h // group], vv[:, h // group]
+            s = torch.where(seen, qh @ kh.T * args["scale"], -math.inf)
+            w = torch.where(seen.any(1, keepdim=True), s.softmax(-1), 0.0)
+            r, a = w @ vh, w @ vh.abs()
+            size = torch.where(seen, qh.abs() @ kh.abs().T, 0.0).amax(-1, keepdim=True) * args["scale"]
+            d = (hd + 4) * U32 * size + 2.0 ** -21
+            if args["q"].dtype == torch.float32:
+                tol = 2 * (d + 2.0 ** -21 * size) * a + (2.0 ** -21 + c * U32) * a + U32 * r.abs()
+            else:
+                tol = 2 * d * a + (U16 + 2.0 ** -14) * a + U16 * r.abs()
+            err = (got[o:o + n, h].double() - r).abs()
+            assert bool((err <= tol * 1.01 + 1e-30).all()), (b, h, float((err / (tol * 1.01 + 1e-30)).max()))
+
+
+@pytest.mark.parametrize("cache", ["bf16", "fp32", "fp8"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (16, 2, 128)])
+@pytest.mark.parametrize("nodes, hists, kind", [([1024, 1000], [0, 700], "none"), ([1024, 1, 513], [1500, 40, 31], "random"),
+                                                ([700, 1024], [64, 3], "tree")])
+def test_tree_attention_of_up_to_1024_rows(cuda_device, cache, heads, nodes, hists, kind):
+    """The pieces in which a prompt is read, and the largest trees."""
+    args, *lens = attention_case(cache, heads, nodes, hists, 16, kind, 51, cuda_device)
+    status = ops.status_tensor(cuda_device)
+    ws = ops.Workspace(cuda_device)
+    got = ops.tree_attention(**args, workspace=ws, status=status)
+    check_on_device(args, *lens, got)
+    assert int(status) == 0 and int(ws.buf[:65536 if ws.buf.numel() > 65536 else 0].sum()) == 0
+    assert torch.equal(ops.tree_attention(**args, workspace=ws), got)
+
+
+def test_a_prompt_in_pieces_over_the_8_bit_cache(cuda_device):
+    """A prompt written and attended in pieces of 1024, 1024 and 500: every piece's rows are those of one causal
+    attention over what the cache holds."""
+    nq, nkv, hd, bs, n = 8, 2, 64, 16, 2548
+    g = torch.Generator().manual_seed(7)
+    pools = [torch.zeros(n // bs + 2, bs, nkv, hd, dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.full((n // bs + 2, bs, nkv), 127, dtype=torch.uint8, device=cuda_device) for _ in range(2)]
+    table = torch.randperm(n // bs + 2, generator=g)[:-(-n // bs)].to(torch.int32)[None].to(cuda_device)
+    angle = torch.arange(float(n))[:, None] * 1e4 ** (-torch.arange(0, hd, 2) / hd)
+    cos, sin = angle.cos().to(cuda_device), angle.sin().to(cuda_device)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    ws, start = ops.Workspace(cuda_device), 0
+    for m in (1024, 1024, 500):
+        qkv = torch.randn(m, (nq + 2 * nkv) * hd, generator=g).to(torch.bfloat16).to(cuda_device)
+        pos = torch.arange(start, start + m, dtype=torch.int32, device=cuda_device)
+        slots = table[0][(pos // bs).long()] * bs + pos % bs
+        q = torch.empty(m, nq, hd, dtype=torch.bfloat16, device=cuda_device)
+        ops.qkv_rope_append_fp8(qkv, pos, slots.to(torch.int32), cos, sin, q, *pools, *scales, nq, nkv, hd)
+        args = dict(q=q, pool_k_layer=pools[0], pool_v_layer=pools[1], block_tables=table, ctx_lens=i32(start + m),
+                    q_lens=i32(m), q_offsets=i32(0), max_q_len=m, max_ctx=start + m, scale=hd ** -0.5, tree_mask=None,
+                    k_scale=scales[0], v_scale=scales[1])
+        check_on_device(args, [start + m], [m], [0], ops.tree_attention(**args, workspace=ws))
+        start += m
