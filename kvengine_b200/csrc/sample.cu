@@ -161,11 +161,11 @@ __device__ __forceinline__ const T* row_at(const Rows& r, int row) {
   return static_cast<const T*>(r.second) + (i / r.k) * r.second_sb + (i % r.k) * r.second_sj;
 }
 
-// 1 / T to 2^-46: one fp32 quotient and its remainder, a fraction of a 64-bit division's latency.
+// 1 / T in 64 bits: an fp32 quotient and its remainder, a fraction of a 64-bit division's latency.
 __device__ __forceinline__ double inverse(float t) {
   if (t > 1e30f) return 1.0 / t;  // fp32's quotient would be subnormal
-  const float r = 1.f / t;
-  return (double)r + (double)r * fmaf(-t, r, 1.f);
+  const double r = 1.f / t, e = fma(-(double)t, r, 1.0);  // e of up to 2^-24, exactly
+  return r + r * (e + e * e);
 }
 // log2 of e^(x / T) over e^(b / T) in 64 bits, b a row's largest logit (an infinite one: only its likes count).
 __device__ __forceinline__ double exponent(float x, float b, float t) {
