@@ -407,7 +407,7 @@ int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k, const void
  * computed in fp32 and rounded once, to q_out's dtype or to the cache.
  * kve_kv_append_fp8: kve_kv_append for such a cache (rows already rotated).
  * kve_kv_read_fp8: rows of given slots as the values they stand for, k_out and v_out
- * [n_tokens, num_kv_heads, head_dim] in dtype (exact in bf16 and fp32). */
+ * [n_tokens, num_kv_heads, head_dim] in dtype (exact in fp32, and in bf16 from 2^-126 on; below, rounded). */
 int kve_qkv_rope_append_fp8(const void* qkv, int dtype, int n_tokens, int num_heads, int num_kv_heads, int head_dim,
                             const int32_t* positions, const int32_t* slots, const float* rope_cos,
                             const float* rope_sin, int rope_len, void* q_out, void* pool_k, void* pool_v,
@@ -429,8 +429,8 @@ int kve_kv_read_fp8(const void* pool_k, const void* pool_v, const uint8_t* k_sca
  * Uniforms in [0, 1) and Gumbel noise -log(-log u) give tokens distributed as sampling
  * from the target alone. T <= 0 (or NaN): p and q are one-hot at their lowest argmax; a
  * subnormal T counts as 2^-126.
- * A NaN logit counts as minus infinity; a row without any probability accepts nothing
- * and gives token 0 with log-probability -inf. A draft outside [0, vocab) is rejected
+ * A NaN logit counts as minus infinity; for T > 0 a row without any probability accepts
+ * nothing and gives token 0 with log-probability -inf. p and q are good to about 2^-20 of themselves. A draft outside [0, vocab) is rejected
  * and recorded as KVE_ERR_BOUNDS.
  * logits: [batch, k+1, vocab] rows row_stride elements apart (fp32 or bf16); draft_logits
  * (same dtype): row j of sequence b at b * stride_b + j * stride_j; drafts as for

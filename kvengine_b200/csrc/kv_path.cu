@@ -10,8 +10,8 @@
 // A CTA takes some columns of one sequence (the grid spreads layers, K and V and
 // columns), so a batch's few megabytes are spread over all SMs; it is bound by the
 // latency of a load and a store behind each other per eight rows, and, for large
-// batches, by HBM. Measured: 24 layers of e4m3 rows (2 heads of 64), one sequence, 2.2 us; 36 layers of
-// bf16 rows (2 heads of 128), 64 sequences of up to 16 nodes (6.9 MB moved), 5.4 us.
+// batches, by HBM. Measured: 24 layers of e4m3 rows (2 heads of 64), one sequence, 1.9 us in a replayed graph
+// (3.4 a call, host time); 36 layers of bf16 rows (2 heads of 128), 64 sequences of up to 16 nodes (6.9 MB moved), 5.1 us.
 #include "kve_common.cuh"
 
 namespace kve {

@@ -23,7 +23,7 @@
 // shared memory.
 //
 // Measured, vocabulary 151936: 128 chains of 4 fp32 drafts with the draft's logits (778 MB) 141 us, 64 trees of
-// 16 bf16 nodes (350 MB) 75 us, one bf16 chain 13 us. The first kernel takes three quarters of
+// 16 bf16 nodes (350 MB) 76 us, one bf16 chain 13.5 us (replayed graphs). The first kernel takes three quarters of
 // the large ones, at 83 % of HBM's throughput; one chain is two kernels' latencies.
 //
 // Precision: a row is held as (b, z), z = sum 2^((x - b) c) with c = log2(e) / T and b the

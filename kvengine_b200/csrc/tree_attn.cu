@@ -35,8 +35,10 @@
 //         infinities among their operands are computed again, key by key.
 // Scores, maxima, sums and outputs are fp32 throughout.
 //
-// Measured: fp32, 14 / 2 heads of 64, one tree of 9 nodes behind 131 keys, 9.1 us (27 us before row
-// blocks shrank to spread a small grid): latency, a few tiles a warp behind each other.
+// Measured: fp32, 14 / 2 heads of 64, one tree of 9 nodes behind 131 keys, 9.2 us (27 us before row
+// blocks shrank to spread a small grid): latency, one tile a warp in 24 CTAs (lengths, table, tile, products one after
+// the other), the merge of the warps and then of three chunks through memory. 64 trees of 16 nodes, 16 / 2 heads
+// of 128, 175 to 700 keys, 322 us: one CTA an SM, three products and the splitting of K and V for every element.
 #include <cuda_fp8.h>
 #include <math.h>
 

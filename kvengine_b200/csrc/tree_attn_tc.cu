@@ -30,11 +30,12 @@
 // 0 x V would spread to rows that do not see them. Where there are any, the chunk's rows
 // are computed again, key by key.
 //
-// Measured, 16 / 2 heads of 128: 32 trees of 64 nodes at 4500 keys 80 us (950 TFLOP/s), 64 of 16 nodes
-// at 175 to 700 keys 14.4 us; over e4m3 caches 261 us (the copying warps' chains of loads, conversions and stores) and,
-// at 700 keys, 41 us (707 and 78 us in the kernel of tree_attn.cu). The wide case is bound by
-// the softmax warps' issue slots; running every kShare-th pair of exponentials on
-// the fp32 units takes 81.7 us at 4, 85.7 at 2, and 87.2 with none.
+// Measured (replayed graphs), 16 / 2 heads of 128: 32 trees of 64 nodes at 4500 keys 81 us (930 TFLOP/s), 64 of 16 nodes
+// at 175 to 700 keys 15.8 us; over e4m3 caches 265 us (the copying warps' chains of loads, conversions and stores) and,
+// at 700 keys, 44 us (707 and 78 us in the kernel of tree_attn.cu). In the wide case no unit is saturated: the tensor
+// cores are busy in half of the cycles, the schedulers issue in 45 % of them, the exponentials' unit runs at 38 %; a step
+// is the chain product, softmax, product with two tiles a group in flight, on 128 of the 148 SMs. Running every kShare-th
+// pair of exponentials on the fp32 units takes 81.7 us at 4, 85.7 at 2, and 87.2 with none.
 #include <cuda_fp8.h>
 #include <float.h>
 #include <math.h>
