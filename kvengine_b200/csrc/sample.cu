@@ -445,7 +445,7 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
   float low = -INFINITY, high = -INFINITY, other = -INFINITY;  // its bounds, and the others' largest upper bound
   __syncthreads();
   if (p.z > 0.0 && !slow) {
-    // Keys times z here. Exponents are fused from x c and relative to b c as rounded;
+    // Keys times z here, their exponents fused from x c and relative to b c as rounded.
     const float off = -(p.b * c), qoff = -(q.b * c);
     volatile int* bar = &sh.bar;
     // Upper bounds without the draft are u = e + g (1 + 8 kOff). A key k = e + g, e at most 0, is at most

@@ -5,12 +5,14 @@ Tolerances as in test_gpu_tree_sampling.py, which derives them.
 """
 
 import math
+import random
 
 import pytest
 import torch
 
-from kvengine_b200 import ops
-from test_gpu_tree_sampling import U16, U32, attention_case, check_attention, plain_chain, plain_tree, same_logprobs, values
+from kvengine_b200 import PagedKVCache, ops
+from test_gpu_tree_sampling import (U16, U32, attention_case, check_attention, plain_chain, plain_tree, same_logprobs,
+                                    tree_inputs, values)
 
 pytestmark = pytest.mark.gpu
 
@@ -380,3 +382,77 @@ def test_a_prompt_in_pieces_over_the_8_bit_cache(cuda_device):
                     k_scale=scales[0], v_scale=scales[1])
         check_on_device(args, [start + m], [m], [0], ops.tree_attention(**args, workspace=ws))
         start += m
+
+
+# ---------------------------------------------------------------- a captured step
+@pytest.mark.parametrize("cache", ["bf16", "fp8"])
+def test_a_whole_step_captured_and_replayed(cuda_device, cache):
+    """Rows written, attended, verified and moved together in one graph on a side stream, with one workspace for all: replays
+    with new inputs leave what the same calls leave outside a graph."""
+    dev, nq, nkv, hd, bs, layers, V = cuda_device, 14, 2, 64, 16, 3, 3000
+    g, rng = torch.Generator().manual_seed(4), random.Random(4)
+    trees = [[-1, 0, 0, 1, 1, 3, 5], [-1, 0, 1, 1, 2], [-1]]
+    nodes, hist, off = [7, 5, 1], [900, 30, 77], [0, 7, 12, 13]
+    fp8, dt, n = cache == "fp8", torch.bfloat16, 13
+    pools = []
+    for _ in range(2):
+        pool = PagedKVCache(layers, nkv, hd, 70, bs, torch.float8_e4m3fn if fp8 else dt, dev)
+        for x in (pool.k, pool.v):
+            x.copy_((torch.randn(x.shape, generator=torch.Generator().manual_seed(8)) * 2).to(x.dtype))
+        pools.append(pool)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    ids = list(range(70))
+    rng.shuffle(ids)
+    table = torch.zeros(3, 57, dtype=torch.int32)
+    for b, (h, m) in enumerate(zip(hist, nodes)):
+        k = -(-(h + m) // bs)
+        table[b, :k] = torch.tensor([ids.pop() for _ in range(k)])
+    slots = i32([int(table[b, p // bs]) * bs + p % bs for b in range(3) for p in range(hist[b], hist[b] + nodes[b])])
+    pos = i32([h + i for h, m in zip(hist, nodes) for i in range(m)])
+    angle = torch.arange(1000.0)[:, None] * 1e4 ** (-torch.arange(0, hd, 2) / hd)
+    cos, sin, mask = angle.cos().to(dev), angle.sin().to(dev), ops.tree_mask_words(trees).to(dev)
+    fixed = [table.to(dev), i32([h + m for h, m in zip(hist, nodes)]), i32(nodes), i32(off), i32(hist), i32(sum(trees, []))]
+
+    def fresh():
+        logits, tokens, u = tree_inputs(trees, V, dt, g, rng)
+        return [torch.randn(layers, n, (nq + 2 * nkv) * hd, generator=g).to(dt), logits, tokens, u * 0.005, gumbels(3, V, g=g),
+                torch.tensor([0.8, 0.0, 1.2])]
+
+    def step(pool, x, ws, q):
+        outs = []
+        for layer in range(layers):
+            into = [pool.k[layer], pool.v[layer]]
+            scales = [pool.k_scale[layer], pool.v_scale[layer]] if fp8 else []
+            (ops.qkv_rope_append_fp8 if fp8 else ops.qkv_rope_append)(x[0][layer], pos, slots, cos, sin, q, *into, *scales, nq, nkv, hd)
+            outs.append(ops.tree_attention(q, *into, *fixed[:4], 7, 907, hd ** -0.5, mask, *scales, workspace=ws))
+        res = ops.tree_sample_accept(x[1], x[2], fixed[5], fixed[2], fixed[3], 7, x[3], x[4], x[5], workspace=ws)
+        ops.kv_commit_path(pool.k, pool.v, fixed[0], fixed[4], res[1], res[0], pool.k_scale, pool.v_scale)
+        return outs + list(res)
+
+    q = torch.empty(n, nq, hd, dtype=dt, device=dev)
+    inputs = [x.to(dev) for x in fresh()]
+    ws = ops.Workspace(dev)
+    ws.get(8 << 20)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    moved = 0
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step(pools[0], inputs, ws, q)
+        for _ in range(3):
+            new = [x.to(dev) for x in fresh()]
+            for x, y in zip(inputs, new):
+                x.copy_(y)
+            graph.replay()
+            want = step(pools[1], new, ops.Workspace(dev), torch.empty_like(q))
+            side.synchronize()
+            for x, y in zip(got, want):
+                assert torch.equal(x, y)
+            for a, b in ((pools[0].k, pools[1].k), (pools[0].v, pools[1].v)):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+            if fp8:
+                assert torch.equal(pools[0].k_scale, pools[1].k_scale) and torch.equal(pools[0].v_scale, pools[1].v_scale)
+            moved += sum(want[layers].tolist())
+    assert moved >= 3  # the numbers accept paths, so that rows move
+    assert int(ws.buf[:65536].sum()) == 0
