@@ -222,9 +222,11 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
   float sum_off = 0.f;                         // relative to this
   auto rebase = [&](float top) {
     if (top > most) {
-      z *= ex2(-off - top * c);  // of nothing at the first
+      // the product rounded, as the terms are relative to it (a fused one would move z by its rounding)
+      const float next = -__fmul_rn(top, c);
+      z *= ex2(next - off);  // of nothing at the first
       most = top;
-      off = -(top * c);
+      off = next;
     }
   };
   auto one = [&](float v, int) {
@@ -275,7 +277,7 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
       if (v != -INFINITY) sum += ex2((float)exponent(v, top, t));
     }
   } else {
-    const float b = top * c;
+    const float b = __fmul_rn(top, c);
     sum = most == -INFINITY ? 0.0 : sum * ex2(-off - b - fmaf(top, c, -b));
   }
   z = (float)sum;
@@ -417,7 +419,7 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
     sh.bar = ordered(-FLT_MAX);  // which minus infinity does not reach
     sh.n = 0;
     // z of p over z of q, for sums relative to b c as rounded
-    if (qrow && !slow) sh.ratio = (float)(p.z / q.z) * ex2(fmaf(p.b, c, -(p.b * c)) - fmaf(q.b, c, -(q.b * c)));
+    if (qrow && !slow) sh.ratio = (float)(p.z / q.z) * ex2(fmaf(p.b, c, -__fmul_rn(p.b, c)) - fmaf(q.b, c, -__fmul_rn(q.b, c)));
   }
   // 16 bytes of logits at a time from their first 16-byte boundary on, and their noise
   const int mis = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
@@ -446,7 +448,7 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
   __syncthreads();
   if (p.z > 0.0 && !slow) {
     // Keys times z here, their exponents fused from x c and relative to b c as rounded.
-    const float off = -(p.b * c), qoff = -(q.b * c);
+    const float off = -__fmul_rn(p.b, c), qoff = -__fmul_rn(q.b, c);
     volatile int* bar = &sh.bar;
     // Upper bounds without the draft are u = e + g (1 + 8 kOff). A key k = e + g, e at most 0, is at most
     // u + 10 kOff |k| + 4 kOff: positive noise brings along more than e can be off by, and with negative noise

@@ -85,6 +85,28 @@ def test_tree_sample_accept_at_any_temperature(cuda_device, dt, kind, temperatur
         same_logprobs(got[3][b:b + 1], [want[3]])
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [3e3, 1e5, -1e6, 1.5e6, 2.9e6, 6e6])
+@pytest.mark.parametrize("V", [5, 2000, 30000])
+def test_sampling_with_logits_far_from_zero(cuda_device, dt, shift, V):
+    """The probabilities are those of the logits' differences, wherever they lie: x c has an ulp of up to 1/2 here, which
+    a thread whose largest logit changes on the way must not lose."""
+    g = torch.Generator().manual_seed(V)
+    B, k = 8, 3
+    target = torch.sort(torch.randn(B, k + 1, V, generator=g) * 3, -1).values if V == 2000 else torch.randn(B, k + 1, V, generator=g) * 3
+    draft = target[:, :k] + torch.randn(B, k, V, generator=g)
+    target, draft = (target + shift).to(dt), (draft + shift).to(dt)
+    t = torch.tensor([0.7, 1.0, 0.99, 1.3, 3.0, 0.5, 0.31, 2.0])
+    drafts = (draft.float() / t[:, None, None] + gumbels(B, k, V, g=g)).argmax(-1).int()
+    u, gumbel = torch.rand(B, k, generator=g), gumbels(B, V, g=g)
+    for dl in (None, draft):
+        want = plain_chain(target, drafts, u, gumbel, t, dl)
+        got = ops.sample_accept(*[x.to(cuda_device) for x in (target, drafts, u, gumbel, t)],
+                                draft_logits=None if dl is None else dl.to(cuda_device))
+        assert got[0].tolist() == want[0] and got[1].tolist() == want[1]
+        same_logprobs(got[2], want[2])
+
+
 def test_sampling_at_an_infinite_temperature(cuda_device):
     """All tokens but those of minus infinity have the same probability."""
     g = torch.Generator().manual_seed(3)
