@@ -32,7 +32,9 @@
 // the rest is small: past |b c| of 2^22 (half an ulp would be an exponent of 1/4, at 3e9 more than fp32's
 // whole range) a row's exponents are (x - b) c from 64-bit differences, more slowly. 2^x runs on ex2.approx (2^-22)
 // into fp32 sums of up to 128 of a thread's vectors, those into a 64-bit one, and the threads' pairwise in
-// fp32 again: p is good to about 2^-21 and 2^-22 times the mean size of the exponents (c's rounding).
+// fp32 again. The largest logit's 1 is kept out of all of them: where it has nearly the whole probability, what p and q
+// leave to the others is what they differ by, and an fp32 sum that begins with 1 loses it below 2^-24. So p is
+// good to (1 - its largest) times 2^-21 and 2^-22 the mean size of the exponents (c's rounding).
 // Acceptance, log-probabilities and every candidate that fp32 does not rule out are computed in 64
 // bits from these sums. A NaN logit counts as minus infinity (never drawn);
 // rows with one are summed again, slowly.
@@ -60,6 +62,12 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // The temperature as it counts: 0 where T <= 0 or NaN, and subnormal numbers as 2^-126 (c stays finite).
 __device__ __forceinline__ float heat(float t) { return t > 0.f ? fmaxf(t, FLT_MIN) : 0.f; }
+// Floats as integers of the same order.
+__device__ __forceinline__ int ordered(float f) {
+  const int i = __float_as_int(f);
+  return i < 0 ? i ^ 0x7fffffff : i;
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i < 0 ? i ^ 0x7fffffff : i); }
 // NaN as minus infinity.
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
 
@@ -86,10 +94,11 @@ template <> struct Pack<__nv_bfloat16> {
 };
 
 // Calls f(value, index) for columns [lo, hi) of a row, 16 bytes at a time from the
-// row's first 16-byte boundary on; `batch(values, first index)` gets the vectors, and `fold()` is
+// row's first 16-byte boundary on; `batch(values, first index)` gets the vectors, `start(U times 16 bytes)` the
+// first U of a warp's threads before (where all have as many), and `fold()` is
 // called now and then in a long row, after every 16 U of a thread's vectors.
-template <typename T, int THREADS, int U, typename Batch, typename One, typename Fold>
-__device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch, One&& one, Fold&& fold) {
+template <typename T, int THREADS, int U, typename Batch, typename One, typename Start, typename Fold>
+__device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch, One&& one, Start&& start, Fold&& fold) {
   constexpr int N = Pack<T>::N;
   const int off = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
   const int head = min(lo + (off ? N - off : 0), hi);
@@ -101,6 +110,7 @@ __device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = __ldcg(v + i + u * THREADS);
+    if (i == (int)threadIdx.x && (i | 31) + (U - 1) * THREADS < nvec) start(raw);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float x[N];
@@ -122,7 +132,7 @@ __device__ __forceinline__ void scan(const T* row, int lo, int hi, Batch&& batch
 }
 
 // What the first kernel leaves of one part of a row: its largest logit, and the sum relative to
-// that or, for T <= 0, its column.
+// that less 1 or, for T <= 0, its column.
 struct Part {
   float b, z;
 };
@@ -198,7 +208,7 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
 #pragma unroll
       for (int j = 0; j < Pack<T>::N; ++j) one(v[j], i + j);
     };
-    scan<T, kStatThreads, 2>(x, lo, hi, batch, one, [] {});
+    scan<T, kStatThreads, 2>(x, lo, hi, batch, one, [](const auto&) {}, [] {});
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float ov = __shfl_xor_sync(0xffffffffu, best, o);
@@ -217,28 +227,40 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
     return;
   }
   const float c = (float)kLog2e / t;
-  float most = -INFINITY, off = 0.f, z = 0.f;  // this thread's largest logit, minus that times c, and its latest terms' sum
-  double sum = 0.0;                            // the others' (a long row's terms are below half an ulp of an fp32 sum),
-  float sum_off = 0.f;                         // relative to this
-  auto rebase = [&](float top) {
-    if (top > most) {
-      // the product rounded, as the terms are relative to it (a fused one would move z by its rounding)
-      const float next = -__fmul_rn(top, c);
-      z *= ex2(next - off);  // of nothing at the first
-      most = top;
-      off = next;
-    }
+  float most = -FLT_MAX, off = 0.f, n = 0.f;  // this thread's largest logit so far, minus that times c, how often it came,
+  float z = 0.f;                              // and the sum of the latest others
+  double sum = 0.0;                           // that of those before (a long row's terms are below half an ulp of an fp32 sum),
+  float sum_off = 0.f;                        // relative to this
+  auto lift = [&](float top) {
+    // the product rounded, as the terms are relative to it (a fused one would move z by its rounding)
+    const float next = -__fmul_rn(top, c);
+    if (most > -FLT_MAX) z = z * ex2(next - off) + n * ex2(fmaf(most, c, next));
+    most = top;
+    off = next;
+    n = 0.f;
   };
   auto one = [&](float v, int) {
-    rebase(v);
-    z += ex2(fmaf(v, c, off));
+    if (v >= most) {
+      if (v > most) lift(v);
+      n += 1.f;
+    } else {
+      z += ex2(fmaf(v, c, off));
+    }
   };
   auto batch = [&](auto& v, int) {
     constexpr int N = Pack<T>::N;
     float top = v[0];
 #pragma unroll
     for (int j = 1; j < N; ++j) top = fmaxf(top, v[j]);  // passes over NaN
-    rebase(top);
+    if (__builtin_expect(top >= most, 0)) {
+      if (top > most) lift(top);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (v[j] == most) {
+          n += 1.f;
+          v[j] = -INFINITY;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = ex2(fmaf(v[j], c, off));
 #pragma unroll
@@ -252,7 +274,21 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
     sum_off = off;
     z = 0.f;
   };
-  scan<T, kStatThreads, 8>(x, lo, hi, batch, one, fold);
+  // A warp starts from the largest of its threads' first vectors: from its own first, nearly every vector
+  // would be a new largest for some thread, and the warp would wait for it.
+  auto start = [&](const auto& raw) {
+    float m = -FLT_MAX;
+#pragma unroll
+    for (int u = 0; u < (int)(sizeof(raw) / sizeof(uint4)); ++u) {
+      float v[Pack<T>::N];
+      Pack<T>::unpack(raw[u], v);
+#pragma unroll
+      for (int j = 0; j < Pack<T>::N; ++j) m = fmaxf(m, v[j]);  // passes over NaN
+    }
+    m = unordered(__reduce_max_sync(0xffffffffu, ordered(m)));
+    if (m > most) lift(m);
+  };
+  scan<T, kStatThreads, 8>(x, lo, hi, batch, one, start, fold);
   // the part's base, then its sum
   auto block_max = [&](float v) {
 #pragma unroll
@@ -265,29 +301,35 @@ row_stats_kernel(Rows rows, int vocab, int chunk, int parts, const float* temper
     return v;
   };
   const float top = block_max(most);
-  fold();
-  const bool odd = __syncthreads_or(!(sum < INFINITY));  // a NaN, or infinite logits
-  if (top == -INFINITY) {
-    sum = 0.0;
+  if (sum != 0.0) z = (float)(sum * ex2(off - sum_off) + z);
+  const bool odd = __syncthreads_or(!(z < INFINITY));  // a NaN, or infinite logits
+  float tops = 0.f;  // how often the part's largest came
+  if (top == -FLT_MAX && !odd && !__syncthreads_or(n > 0.f)) {
+    z = 0.f;  // nothing but minus infinity
   } else if (odd || far(top, c)) {
     // infinite logits share the whole probability, NaN has none
     sum = 0.0;
     for (int i = lo + threadIdx.x; i < hi; i += kStatThreads) {
       const float v = clean(Elem<T>::to_f(x[i]));
-      if (v != -INFINITY) sum += ex2((float)exponent(v, top, t));
+      if (v == top) tops += 1.f;
+      else if (v != -INFINITY) sum += ex2((float)exponent(v, top, t));
     }
-  } else {
-    const float b = __fmul_rn(top, c);
-    sum = most == -INFINITY ? 0.0 : sum * ex2(-off - b - fmaf(top, c, -b));
+    z = (float)sum;
+  } else if (most > -FLT_MAX) {
+    const float b = __fmul_rn(top, c), moved = fmaf(top, c, -b);
+    z *= ex2(-off - b - moved);
+    if (most == top) tops = n;
+    else z += n * ex2(fmaf(most, c, -b) - moved);
   }
-  z = (float)sum;
   z = warp_sum(z);
-  if (lane == 0) sz[warp] = z;
+  // at least 1 where there is any; a few, so that integers do
+  int count = __reduce_add_sync(0xffffffffu, (int)tops);
+  if (lane == 0) { sz[warp] = z; sm[warp] = __int_as_float(count); }
   __syncthreads();
   if (warp == 0) {
-    z = lane < kStatThreads / 32 ? sz[lane] : 0.f;
-    z = warp_sum(z);
-    if (lane == 0) out[(size_t)row * parts + part] = Part{top, z};
+    z = warp_sum(lane < kStatThreads / 32 ? sz[lane] : 0.f);
+    count = __reduce_add_sync(0xffffffffu, lane < kStatThreads / 32 ? __float_as_int(sm[lane]) : 0);
+    if (lane == 0) out[(size_t)row * parts + part] = Part{count ? top : -INFINITY, (float)(count - 1) + z};
   }
 }
 
@@ -316,7 +358,7 @@ __device__ __forceinline__ void join_rows(const Part* parts, int n_parts, int gr
       r.arg = sub < n_parts && p.b == b ? __float_as_int(p.z) : 0x7fffffff;
       for (int o = 1; o < group; o <<= 1) r.arg = min(r.arg, __shfl_xor_sync(0xffffffffu, r.arg, o));
     } else {
-      r.z = p.b == -INFINITY ? 0.0 : p.b == b ? (double)p.z : (double)p.z * exp2(exponent(p.b, b, t));
+      r.z = p.b == -INFINITY ? 0.0 : p.b == b ? 1.0 + p.z : (1.0 + p.z) * exp2(exponent(p.b, b, t));
       for (int o = 1; o < group; o <<= 1) r.z += __shfl_xor_sync(0xffffffffu, r.z, o);
     }
     if (i < n && sub == 0) out[i] = r;
@@ -386,12 +428,6 @@ struct DrawShared {
   int bar;                     // what a column has to reach to be the CTA's best, as an ordered integer
   int n;                       // candidates kept
 };
-__device__ __forceinline__ int ordered(float f) {
-  const int i = __float_as_int(f);
-  return i < 0 ? i ^ 0x7fffffff : i;
-}
-__device__ __forceinline__ float unordered(int i) { return __int_as_float(i < 0 ? i ^ 0x7fffffff : i); }
-
 // What fp32 may be off by, relative to the size of each term of a key or weight: exponents, ex2.approx and
 // lg2.approx are good to 2^-22, and a handful of roundings of 2^-24 come on top.
 constexpr float kOff = 0x1p-20f;

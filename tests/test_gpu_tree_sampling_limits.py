@@ -227,6 +227,44 @@ def test_residual_of_nearly_equal_distributions(cuda_device, dt, eps):
     assert bool((chosen >= bar).all()), int((chosen < bar).sum())
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [5, 300, 30000])
+@pytest.mark.parametrize("temperature", [0.3, 0.1, 0.04, 0.02])
+def test_residual_where_one_token_has_nearly_all(cuda_device, dt, V, temperature):
+    """p and q both give nearly all to the same token, and a draft of the little rest is rejected: that rest decides. The
+    sums hold the largest token's 1 apart, so what p and q are off by, relative to themselves, is that of the others' terms: 2^-21 of
+    their share, and 2^-22 times the exponents' mean size (the largest's is 0). The exponents x / T here, of 64 bits, are off by half
+    an ulp of up to s = max |x| / T each, at x and at the largest: 2^-52 s of p, and 2^-51 for the other roundings. The token
+    drawn is the argmax for some p and q within that; one of no weight to speak of never is."""
+    g = torch.Generator().manual_seed(V)
+    B = 300
+    target = torch.randn(B, 2, V, generator=g)
+    target[:, :, 1] += 5.0
+    draft = target[:, :1] + 0.1 * torch.randn(B, 1, V, generator=g)
+    drafts = 2 + torch.randint(0, V - 2, (B,), generator=g)
+    draft[torch.arange(B), 0, drafts] += 3 * temperature
+    draft[:, 0, 1] += 0.3 * (torch.arange(B) % 3 - 1) * temperature
+    target, draft = target.to(dt), draft.to(dt)
+    u, gumbel, t = torch.full((B, 1), 0.9999), gumbels(B, V, g=g), torch.full((B,), temperature)
+    n, emitted, _ = ops.sample_accept(*[x.to(cuda_device) for x in (target, drafts[:, None].int(), u, gumbel, t)],
+                                      draft_logits=draft.to(cuda_device))
+    temp = float(t[0])
+    p, q = (target[:, 0].double() / temp).softmax(-1), (draft[:, 0].double() / temp).softmax(-1)
+    rejected = (0.9999 * q.gather(1, drafts[:, None]) > 1.001 * p.gather(1, drafts[:, None]))[:, 0]
+    assert int(rejected.sum()) >= B // 2 and bool((n.cpu()[rejected] == 0).all())
+
+    def error(w, x):
+        x = x.double() / temp
+        size = (w * (x.amax(-1, keepdim=True) - x)).sum(-1, keepdim=True) * 1.4427
+        return w * (2.0 ** -21 * (1 - w.amax(-1, keepdim=True)) + 2.0 ** -22 * size + 2.0 ** -51 + 2.0 ** -52 * float(x.abs().max()))
+
+    off = error(p, target[:, 0]) + error(q, draft[:, 0])
+    greatest = ((p - q) + off).clamp(min=0).log() + gumbel.double()
+    bar = (((p - q) - off).clamp(min=0).log() + gumbel.double()).amax(-1)
+    chosen = greatest.gather(1, emitted[:, :1].long().cpu())[:, 0]
+    sure = rejected & (bar > -math.inf)
+    assert int(sure.sum()) >= B // 3 and bool((chosen >= bar)[sure].all()), int((chosen < bar)[sure].sum())
+
 # ---------------------------------------------------------------- the 8-bit cache's scales
 @pytest.mark.parametrize("heads, nodes, bs", [((3, 3, 64), [2, 1], 1), ((4, 1, 128), [2, 1], 7), ((3, 3, 64), [5, 9], 1),
                                               ((6, 1, 128), [9, 4], 7), ((6, 3, 64), [1, 2], 16)])
