@@ -22,8 +22,8 @@
 // from, which is often still in L2; the shares' best tokens meet through distributed
 // shared memory.
 //
-// Measured, vocabulary 151936: 128 chains of 4 fp32 drafts with the draft's logits (778 MB) 141 us, 64 trees of
-// 16 bf16 nodes (350 MB) 76 us, one bf16 chain 13.5 us (replayed graphs). The first kernel takes three quarters of
+// Measured, vocabulary 151936: 128 chains of 4 fp32 drafts with the draft's logits (778 MB) 142 us, 64 trees of
+// 16 bf16 nodes (350 MB) 76 us, one bf16 chain 12.7 us (replayed graphs). The first kernel takes three quarters of
 // the large ones, at 83 % of HBM's throughput; one chain is two kernels' latencies.
 //
 // Precision: a row is held as (b, z), z = sum 2^((x - b) c) with c = log2(e) / T and b the
@@ -533,11 +533,24 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
         top = fmaxf(top, u[j]);  // passes over NaN
       }
       if (!(top >= unordered(*bar))) return;
+      // The greatest first: it raises the bar, and the others seldom reach that (they are then read again, for
+      // one copy of the code instead of N).
+      float bx = 0.f, bg = 0.f;
+      int best = 0;
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (u[j] >= unordered(*bar)) consider(x[j], g[j], u[j], v + j);
+        if (u[j] == top) {
+          bx = x[j];
+          bg = g[j];
+          best = j;
+        }
+      consider(bx, bg, top, v + best);
+      const float now = unordered(*bar);
+      int left = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) left |= (u[j] >= now && j != best) << j;
+      for (; left; left &= left - 1) one(Elem<T>::to_f(row[v + __ffs(left) - 1]), v + __ffs(left) - 1);
     };
-    for (int i = lo + threadIdx.x; i < head; i += kDrawThreads) one(Elem<T>::to_f(row[i]), i);
     constexpr int U = sizeof(T) == 4 ? 4 : 2;
     for (int i0 = threadIdx.x; i0 < nvec; i0 += U * kDrawThreads) {
       uint4 raw[U];
@@ -556,7 +569,12 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
           batch(x, g[u], head + (i0 + u * kDrawThreads) * N);
         }
     }
-    for (int j = head + nvec * N + threadIdx.x; j < hi; j += kDrawThreads) one(Elem<T>::to_f(row[j]), j);
+    // the columns before and behind
+    const int before = head - lo, behind = head + nvec * N;
+    for (int j = threadIdx.x; j < before + hi - behind; j += kDrawThreads) {
+      const int v = j < before ? lo + j : behind + j - before;
+      one(Elem<T>::to_f(row[v]), v);
+    }
   }
   // Column v's key in 64 bits; NaN where its weight rounds to nothing there.
   auto exact = [&](int v, float x) {
