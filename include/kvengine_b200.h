@@ -407,7 +407,8 @@ int kve_paged_tree_attn(const void* q, int dtype, const void* pool_k, const void
  * computed in fp32 and rounded once, to q_out's dtype or to the cache.
  * kve_kv_append_fp8: kve_kv_append for such a cache (rows already rotated).
  * kve_kv_read_fp8: rows of given slots as the values they stand for, k_out and v_out
- * [n_tokens, num_kv_heads, head_dim] in dtype (exact in fp32, and in bf16 from 2^-126 on; below, rounded). */
+ * [n_tokens, num_kv_heads, head_dim] in dtype (exact in fp32, and in bf16 from 2^-126
+ * on; below, rounded). */
 int kve_qkv_rope_append_fp8(const void* qkv, int dtype, int n_tokens, int num_heads, int num_kv_heads, int head_dim,
                             const int32_t* positions, const int32_t* slots, const float* rope_cos,
                             const float* rope_sin, int rope_len, void* q_out, void* pool_k, void* pool_v,
@@ -430,8 +431,8 @@ int kve_kv_read_fp8(const void* pool_k, const void* pool_v, const uint8_t* k_sca
  * from the target alone. T <= 0 (or NaN): p and q are one-hot at their lowest argmax; a
  * subnormal T counts as 2^-126.
  * A NaN logit counts as minus infinity; for T > 0 a row without any probability accepts
- * nothing and gives token 0 with log-probability -inf. p and q are good to about 2^-20 of themselves. A draft outside [0, vocab) is rejected
- * and recorded as KVE_ERR_BOUNDS.
+ * nothing and gives token 0 with log-probability -inf. p and q are good to about 2^-20 of
+ * themselves. A draft outside [0, vocab) is rejected and recorded as KVE_ERR_BOUNDS.
  * logits: [batch, k+1, vocab] rows row_stride elements apart (fp32 or bf16); draft_logits
  * (same dtype): row j of sequence b at b * stride_b + j * stride_j; drafts as for
  * kve_greedy_accept; uniforms [batch, k] rows uniform_stride_b apart; gumbel
@@ -461,8 +462,9 @@ int kve_sample_accept(const void* logits, int dtype, int64_t row_stride, const v
  * KVE_ERR_BOUNDS. max_q_len <= 1024.
  * Outputs: n_accepted [batch] (-1 for a sequence without nodes, and, recorded as
  * KVE_ERR_BOUNDS, for one whose length or rows do not fit or, by offsets that do not ascend, got
- * another sequence's temperature; its other outputs are not written), and, [batch, max_q_len]: path (the accepted nodes, node 0 first, then
- * -1), emitted (their tokens without node 0's, the token drawn, then -1), logprobs. */
+ * another sequence's temperature; its other outputs are not written), and,
+ * [batch, max_q_len]: path (the accepted nodes, node 0 first, then -1), emitted (their
+ * tokens without node 0's, the token drawn, then -1), logprobs. */
 size_t kve_tree_sample_accept_workspace_bytes(int n_rows, int vocab);
 int kve_tree_sample_accept(const void* logits, int dtype, int64_t row_stride, const int32_t* tokens,
                            const int32_t* parents, const int32_t* q_lens, const int32_t* q_offsets,

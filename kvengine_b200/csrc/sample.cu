@@ -488,7 +488,8 @@ __device__ __forceinline__ Best draw_columns(DrawShared& sh, int lo, int hi, con
     volatile int* bar = &sh.bar;
     // Upper bounds without the draft are u = e + g (1 + 8 kOff). A key k = e + g, e at most 0, is at most
     // u + 10 kOff |k| + 4 kOff: positive noise brings along more than e can be off by, and with negative noise
-    // neither term is larger than k. So a column with u below bar - 16 kOff (|bar| + 1) is below the bar, and that is what sh.bar holds.
+    // neither term is larger than k. So a column with u below bar - 16 kOff (|bar| + 1) is below the bar, and that
+    // is what sh.bar holds.
     constexpr float kMore = kL * (1.f + 8.f * kOff);
     auto consider = [&](float x, float g, float u, int v) {
       if (!(x > -INFINITY)) return;

@@ -714,7 +714,8 @@ tree_attn_kernel(TreeParams p) {
   // An infinity or a number next to the largest has no two halves (infinity minus infinity): rows that
   // came out as not finite are computed again without them.
   if (KV == kF32 && __syncthreads_or(nan))
-    attend_by_key<QT, false, HD, kThreads>(p, b, h, qoff, hist, key_lo, key_hi, row0, rows, warp, lane, live > 1, part0 + (size_t)c * (RB * 16) * PROW);
+    attend_by_key<QT, false, HD, kThreads>(p, b, h, qoff, hist, key_lo, key_hi, row0, rows, warp, lane, live > 1,
+                                           part0 + (size_t)c * (RB * 16) * PROW);
   if (live == 1) return;
 
   // The last of the tile's chunks to arrive joins them, in chunk order.

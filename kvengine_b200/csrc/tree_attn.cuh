@@ -86,13 +86,14 @@ __device__ __forceinline__ uint32_t chain_bits(int node, int j0) {
 // formula does not, infinities among them. A warp a row, HD / 32 dims a lane. Into `out`, or, where
 // the keys are split, as [row][HD + 4] partials with m and l behind the dims into `part`. Q: of q, out and, but for FP8, the cache.
 template <typename Q, bool FP8, int HD, int THREADS>
-__device__ __forceinline__ void attend_by_key(const TreeParams& p, int b, int h, int qoff, int hist, int key_lo, int key_hi, int row0,
-                                              int rows, int warp, int lane, bool split, float* part) {
+__device__ __forceinline__ void attend_by_key(const TreeParams& p, int b, int h, int qoff, int hist, int key_lo, int key_hi,
+                                              int row0, int rows, int warp, int lane, bool split, float* part) {
   constexpr int DPL = HD / 32;
   const int32_t* table = p.tables + (size_t)b * p.table_stride;
   auto element = [](const void* pool, const uint8_t* scales, size_t row, int d) {
     if constexpr (FP8)
-      return scale_value(scales[row]) * __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(pool)[row * HD + d], __NV_E4M3)));
+      return scale_value(scales[row]) *
+             __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(pool)[row * HD + d], __NV_E4M3)));
     else
       return Elem<Q>::to_f(static_cast<const Q*>(pool)[row * HD + d]);
   };

@@ -841,7 +841,8 @@ tree_attn_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
   }
   if (!failed && recompute) {
-    attend_by_key<__nv_bfloat16, FP8, HD, threads_of(FP8)>(p, b, h, qoff, hist, key_lo, key_hi, row0, rows, warp, lane, live > 1, part);
+    attend_by_key<__nv_bfloat16, FP8, HD, threads_of(FP8)>(p, b, h, qoff, hist, key_lo, key_hi, row0, rows, warp, lane,
+                                                           live > 1, part);
   }
   tc_before();
   __threadfence();
